@@ -21,7 +21,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libdecdec_b200.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CU_SOURCES = ["host.cu", "k_dec.cu", "k_bcq.cu", "k_anyprec.cu", "k_sqllm.cu", "noalloc.cu", "tp_allreduce.cu"]
+CU_SOURCES = ["host.cu", "k_dec.cu", "k_bcq.cu", "k_anyprec.cu", "k_sqllm.cu", "noalloc.cu", "tp_allreduce.cu",
+              "k_kv4.cu", "k_kv4_attn.cu", "k_kv4_decode64.cu", "k_kv4_decode128.cu", "k_kv4_decode256.cu"]
 
 
 def _run(cmd, log=None):
@@ -55,7 +56,7 @@ def build_lib(verbose: bool = False, force: bool = False) -> Path:
                 cmd[1:1] = ["-Xptxas", "-v"]
             jobs.append(cmd)
     logs = []
-    with ThreadPoolExecutor(max_workers=min(6, max(1, len(jobs)))) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         list(ex.map(lambda c: _run(c, logs), jobs))
     if verbose:
         print("\n".join(logs))

@@ -42,6 +42,7 @@ def _load():
 lib = _load()
 
 _vp, _u32, _i, _up, _ll = C.c_void_p, C.c_uint32, C.c_int, C.c_size_t, C.c_longlong
+_f, _rows = C.c_float, [C.c_void_p, C.c_longlong, C.c_longlong]
 
 SIGNATURES = {
     "decdec_last_error": (C.c_char_p, []),
@@ -76,6 +77,13 @@ SIGNATURES = {
     "decdec_dummy_anyprec": (_i, [_vp, _vp, _vp, _u32, _vp, _u32, _u32, _i, _i, _i, _ll, _vp]),
     "decdec_dummy_lutgemm": (_i, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _i, _i, _i, _i, _ll, _vp]),
     "decdec_dummy_sqllm": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _i, _i, _i, _ll, _vp]),
+    "decdec_rotary": (_i, [*_rows, _u32, *_rows, _u32, *_rows, *_rows, _vp, _i, _vp, _u32, _u32, _u32, _i, _f, _i, _vp]),
+    "decdec_kv4_plan": (_i, [_vp, _vp, _u32, _vp, _ll, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "decdec_kv4_append": (_i, [*_rows, *_rows, _vp, _i, _u32, _vp, _u32, _u32, _u32, _u32, _u32, _i, _vp]),
+    "decdec_kv4_gather": (_i, [_vp, _u32, _u32, _u32, _u32, _u32, _vp, _i, _u32, _vp, _vp, _i, _vp]),
+    "decdec_kv4_attention_workspace": (_i, [_u32, _u32, _u32, _u32, _u32, _u32, _u32, _i, C.POINTER(_up)]),
+    "decdec_kv4_attention": (_i, [*_rows, *_rows, _vp, _vp, _u32, _u32, _vp, _ll, _u32, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _f, _u32,
+                                  _i, _vp, _up, _i, _vp]),
 }
 
 for _name, (_res, _args) in SIGNATURES.items():

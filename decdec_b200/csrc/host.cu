@@ -2,6 +2,7 @@
 // launch geometry.  Mirrors the host launchers of the reference (decdec_extension/decdec.cu,
 // dec_config.cu, dec_context.cu) behind plain-C entry points; no torch types.
 #include "internal.h"
+#include "kv4.cuh"
 #include "../../include/decdec_b200.h"
 
 #include <cstdarg>
@@ -72,6 +73,9 @@ std::map<int, std::pair<cudaStream_t, std::pair<cudaEvent_t, cudaEvent_t>>> g_si
 // fails until decdec_stream_reset, instead of computing on top of an unfinished result.
 int check_ws(const Workspace& w) {
     const unsigned code = w.err_host ? *w.err_host : 0u;
+    if (code == kErrKv4Page)
+        return fail(DECDEC_E_DEVICE, "an earlier launch on this stream met a page, a slot or a length outside the 4-bit cache (device code %u); "
+                                     "read it with decdec_stream_status and clear it with decdec_stream_reset", code);
     if (code)
         return fail(DECDEC_E_DEVICE, "an earlier launch on this stream gave up waiting (device code %u); read it with "
                                      "decdec_stream_status and clear it with decdec_stream_reset", code);
@@ -531,6 +535,14 @@ int run_dummy(int dummy_sm, long long iters, void* stream, F gemv) {
 namespace dd {
 // lets other translation units of the library record the message returned by decdec_last_error()
 int set_last_error(int code, const char* msg) { return fail(code, "%s", msg); }
+
+// the device's view of the stream's error word, for kernels that need nothing else of the workspace
+int stream_error_word(cudaStream_t s, unsigned** err) {
+    Workspace ws;
+    if (int r = get_workspace(s, &ws)) return r;
+    *err = ws.err;
+    return 0;
+}
 }  // namespace dd
 
 extern "C" {

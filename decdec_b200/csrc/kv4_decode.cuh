@@ -1,0 +1,719 @@
+// Attention of a few queries over the 4-bit cache (decoding, drafted tokens).
+//
+// softmax(q k^T s) v with k, v = middle + step * (code - 8), middle = offset + 8 step, never formed: with c = code - 8 as tensor-core
+// factors
+//   scores      q.k = sum_g step_g (q_g . c_g) + middle_g (1 . q_g)                per token and group g of the head
+//   outputs     p v = sum_t (p_t step_t) c_t + sum_t p_t middle_t
+// so the codes are the only operands made from the cache: a mask and an OR turn two codes of a word into fp16 numbers 1024 + code (or
+// 1024 + 16 code), one fused multiply-add into code - 8, exact.  (The masked word alone is a pair of subnormal fp16 numbers code * 2^-24
+// and would save that instruction, but the tensor cores align subnormal products ten bits too high: scores lost 2^-14 of their terms.  And
+// codes of one sign make sums that grow with the context and are cut off in one direction at every step.)  Tokens are the 16 rows of
+// an operand in the scores (m16n8k16, 8 queries wide) and its depth in the outputs, so a batch-1 token with 4 queries per key head
+// fills half of each instruction instead of a quarter.
+//   queries     fp16 after scaling each row to a power of two near 2^13: exact for both 16-bit types (elements below 2^-27 of the row's
+//               largest lose bits)
+//   weights     p_t * step_t in fp16 with the steps scaled by a running power of two per group, so that neither small steps nor
+//               small weights become subnormal before they are 2^-23 of the largest
+//   the rest    (scores, running maximum and sum, the middles' part, sums over thread blocks) in fp32
+//
+// The work is a line of cells (16 tokens of one key head), request by request, and every thread block takes an equal part of it
+// (lengths are on the device: each block sums them itself).  A warp streams its own cells through shared memory (cp.async, kStages
+// cells ahead) and keeps its own running maximum and sums; the four warps of a block are added where a segment (one request, head and
+// tile of 8 or 16 query rows) ends.  A segment that blocks share leaves its parts in `part`, and kv4_join adds them.
+#pragma once
+#include "kv4.cuh"
+
+namespace dd {
+
+constexpr int kDecodeThreads = 128;
+constexpr int kDecodeWarps = 4;
+constexpr float kGrow = 4.0f;          // a running maximum follows once it is 2^4 behind
+
+// one part of a cut segment: [rows of a tile][D] sums, then [rows][2] maximum (log2 units) and sum
+__host__ __device__ constexpr uint32_t kv4_part_floats(uint32_t d, uint32_t nt) { return 8u * nt * (d + 2u); }
+
+// how many parts, and of which segment, the block that began a cut segment leaves behind
+struct Kv4Cut {
+    uint32_t parts;                    // 0: this block cut no segment that it began
+    uint32_t request, row0, head;      // row0: first row of the tile among the request's rows
+    uint32_t start, rows;              // first token of the request among all, rows of the request
+};
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 16 bytes into shared memory, zeros where `bytes` is 0
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }     // -126 <= e <= 127
+
+// the codes of a word less 8, as fp16 pairs: (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ void code_pairs(uint32_t x, uint32_t (&h)[4]) {
+    const __half2 low = __float2half2_rn(-1032.0f), by = __float2half2_rn(0.0625f), high = __float2half2_rn(-72.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t y = i < 2 ? x : x >> 8;
+        const uint32_t m = (y & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+        const __half2 v = *reinterpret_cast<const __half2*>(&m);
+        const __half2 r = i & 1 ? __hfma2(v, by, high) : __hadd2(v, low);
+        h[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
+// N consecutive 32-bit words of shared memory, in the widest loads
+template <int N> __device__ __forceinline__ void load_words(uint32_t (&x)[N], const uint8_t* at) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(at + 4 * i);
+            x[i] = u.x; x[i + 1] = u.y; x[i + 2] = u.z; x[i + 3] = u.w;
+        }
+    } else if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(at);
+        x[0] = u.x; x[1] = u.y;
+    } else {
+        x[0] = *reinterpret_cast<const uint32_t*>(at);
+    }
+}
+
+// what a request asks for
+struct Kv4Request {
+    int start, queries, length;        // first row, rows, tokens in the cache
+    int first, cells;                  // cells that some query sees: first, number (at least one)
+    int tiles;                         // tiles of query rows
+};
+
+__device__ __forceinline__ Kv4Request kv4_request(const Kv4Attn& p, uint32_t b, int tile_rows, bool report) {
+    Kv4Request r;
+    const int rows = (int)p.rows;
+    r.start = min(max(p.starts[b], 0), rows);
+    r.queries = max(min(max(p.starts[b + 1], 0), rows) - r.start, 0);
+    r.length = max(p.lengths[b], 0);
+    const long long most = (long long)p.table_cols * p.page_cells * kCellTokens;
+    if ((long long)r.length > most) {
+        if (report) raise_error(p.err, kErrKv4Page);
+        r.length = (int)most;
+    }
+    r.first = p.window ? max(0ll, (long long)r.length - r.queries - (long long)p.window + 1) / kCellTokens : 0;
+    r.cells = max(1, (r.length + kCellTokens - 1) / kCellTokens - r.first);
+    r.tiles = (int)(((long long)r.queries * p.ratio + tile_rows - 1) / tile_rows);
+    return r;
+}
+
+template <int D, int NT> struct DecodeShape {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kRowStride = D + 4;            // floats; keeps the warps' 16-byte stores apart by banks
+    static constexpr int kMergeFloats = kDecodeWarps * kRows * (kRowStride + 2);
+};
+template <int D, int GS> __host__ __device__ constexpr int decode_stages() { return kv4_cell_bytes(D, GS) > 2600 ? 3 : 4; }
+template <int D, int GS, int NT> __host__ __device__ constexpr size_t decode_smem() {
+    return (size_t)kDecodeWarps * decode_stages<D, GS>() * kv4_cell_bytes(D, GS) + DecodeShape<D, NT>::kMergeFloats * 4u;
+}
+
+template <int D, int GS, int NT, int DT>
+__global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
+    using T = typename Tr<DT>::T;
+    using Sh = DecodeShape<D, NT>;
+    constexpr int NG = D / GS;                  // groups of a head
+    constexpr int NW = D / 32;                  // words of 32 elements
+    constexpr int STAGES = decode_stages<D, GS>();
+    constexpr uint32_t CELL = kv4_cell_bytes(D, GS);
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long s_sum[kDecodeThreads / 32];
+    __shared__ long long s_rest;
+    __shared__ uint32_t s_request;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int gid = lane >> 2, tig = lane & 3;
+    uint8_t* ring = smem + (size_t)warp * STAGES * CELL;
+    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+    float* merge = reinterpret_cast<float*>(smem + (size_t)kDecodeWarps * STAGES * CELL);     // [warp][row][kRowStride]
+    float* merge_ml = merge + kDecodeWarps * Sh::kRows * Sh::kRowStride;                      // [warp][row][2]
+    uint8_t* after = reinterpret_cast<uint8_t*>(p.part + (size_t)gridDim.x * 2u * kv4_part_floats(D, NT));
+    Kv4Cut* cuts = reinterpret_cast<Kv4Cut*>(after);
+
+    pdl_trigger();
+    pdl_wait();
+
+    // ---- this block's part of the line of cells
+    const uint32_t run = (p.requests + kDecodeThreads - 1u) / kDecodeThreads;
+    const uint32_t rb0 = min(tid * run, p.requests), rb1 = min(rb0 + run, p.requests);
+    long long mine = 0;
+    for (uint32_t b = rb0; b < rb1; ++b) {
+        const Kv4Request r = kv4_request(p, b, Sh::kRows, blockIdx.x == 0);
+        mine += (long long)r.tiles * p.kv_heads * r.cells;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const long long n = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += n;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) {
+        if (w < warp) before += s_sum[w];
+        total += s_sum[w];
+    }
+    // at least two cells a warp: a shorter part would spend its time in the joining of the parts
+    const long long per = max((total + gridDim.x - 1) / gridDim.x, 2ll * kDecodeWarps);
+    const long long x0 = (long long)blockIdx.x * per, x1 = min(x0 + per, total);
+    const long long excl = before + incl - mine;
+    if (x0 < x1 && excl <= x0 && x0 < excl + mine) {
+        long long at = excl;
+        uint32_t b = rb0;
+        for (;; ++b) {                                       // ends: x0 lies below the end of this run
+            const Kv4Request r = kv4_request(p, b, Sh::kRows, false);
+            const long long n = (long long)r.tiles * p.kv_heads * r.cells;
+            if (x0 < at + n) break;
+            at += n;
+        }
+        s_request = b;
+        s_rest = x0 - at;
+    }
+    __syncthreads();
+    if (p.fill_tail) {
+        const int used = p.requests ? min(max(p.starts[p.requests], 0), (int)p.rows) : 0;
+        for (int t = used + (int)blockIdx.x; t < (int)p.rows; t += gridDim.x) {
+            for (uint32_t e = tid; e < p.kv_heads * p.ratio * D; e += kDecodeThreads)
+                reinterpret_cast<T*>(p.out)[(long long)t * p.out_token + (long long)(e / D) * p.out_head + e % D] = Tr<DT>::from_f(0.0f);
+            if (p.lse)
+                for (uint32_t e = tid; e < p.kv_heads * p.ratio; e += kDecodeThreads) p.lse[(size_t)t * p.kv_heads * p.ratio + e] = -INFINITY;
+        }
+    }
+    Kv4Cut cut = {};
+    if (x0 < x1) {
+        uint32_t b = s_request;
+        Kv4Request rq = kv4_request(p, b, Sh::kRows, false);
+        long long rest = s_rest;
+        int item = (int)(rest / rq.cells);                   // tile * kv_heads + head
+        int c0 = (int)(rest % rq.cells);
+        long long x = x0;
+        while (x < x1) {
+            const int c1 = (int)min((long long)rq.cells, c0 + (x1 - x));
+            const uint32_t head = (uint32_t)item % p.kv_heads;
+            const int row0 = (int)((uint32_t)item / p.kv_heads) * Sh::kRows;
+            const int all_rows = rq.queries * (int)p.ratio;
+
+            // ---- queries of the tile as operands: lane (gid, tig) holds row gid, elements 32 w + 8 tig .. + 7
+            uint32_t qf[NT][NW][4];                          // pairs (0,4), (1,5), (2,6), (3,7)
+            float sf[NT][2], qs[NT][2][NG];                  // of the rows 2 tig, 2 tig + 1 that this lane meets in the sums
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int row = row0 + 8 * nt + gid;
+                const bool live = row < all_rows;
+                const int tok = rq.start + (live ? row / (int)p.ratio : 0);
+                const T* src = reinterpret_cast<const T*>(p.q.p) + (long long)tok * p.q.token + (long long)(head * p.ratio + (live ? row % (int)p.ratio : 0)) * p.q.head;
+                float v[NW][8];
+                float most = 0.0f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    uint4 raw = make_uint4(0, 0, 0, 0);
+                    if (live) {
+                        if (p.q_vec) {
+                            raw = *reinterpret_cast<const uint4*>(src + 32 * w + 8 * tig);
+                        } else {
+                            uint32_t u[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint16_t* e = reinterpret_cast<const uint16_t*>(src + 32 * w + 8 * tig + 2 * i);
+                                u[i] = (uint32_t)e[0] | (uint32_t)e[1] << 16;
+                            }
+                            raw = make_uint4(u[0], u[1], u[2], u[3]);
+                        }
+                    }
+                    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = unpack2<DT>(u[i]);
+                        v[w][2 * i] = f.x;
+                        v[w][2 * i + 1] = f.y;
+                        most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                int e = (int)(__float_as_uint(most) >> 23) - 127;      // the row's exponent
+                e = (most > 0.0f && most < INFINITY) ? max(e, -87) : 13;
+                const float up = pow2(13 - e);
+                float sum[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) sum[g] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        v[w][i] *= up;
+                        sum[w * 32 / GS] += v[w][i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) qf[nt][w][i] = half2_bits(v[w][i], v[w][i + 4]);
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+                    sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+                }
+                const float mine_sf = p.scale_log2 * pow2(e - 13);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    sf[nt][i] = __shfl_sync(0xffffffffu, mine_sf, 8 * tig + 4 * i);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) qs[nt][i][g] = __shfl_sync(0xffffffffu, sum[g], 8 * tig + 4 * i);
+                }
+            }
+            // tokens that each of this lane's rows sees: [from, to)
+            int from[NT][2], to[NT][2];
+            const int pos0 = rq.length - rq.queries;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int row = row0 + 8 * nt + 2 * tig + i;
+                    const int pos = pos0 + min(row, all_rows - 1) / (int)p.ratio;
+                    to[nt][i] = max(pos + 1, 0);
+                    from[nt][i] = p.window ? (int)max(0ll, (long long)pos - (long long)p.window + 1) : 0;
+                }
+            // cells between these are seen whole by every row of the tile
+            const int first_pos = pos0 + row0 / (int)p.ratio, last_pos = pos0 + (min(row0 + Sh::kRows, all_rows) - 1) / (int)p.ratio;
+            const int clear_to = max(first_pos + 1, 0), clear_from = p.window ? (int)max(0ll, (long long)last_pos - (long long)p.window + 1) : 0;
+
+            float acc[D / 16][NT][4], off[NT][2][NG], l[NT][2], m[NT][2], fv[NG];
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][nt][j] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                fv[g] = 0.0f;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) off[nt][0][g] = off[nt][1][g] = 0.0f;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) { l[nt][i] = 0.0f; m[nt][i] = -INFINITY; }
+
+            // ---- this warp's cells: c0 + warp, + 4, ...
+            const int count = (c1 - c0 - warp + kDecodeWarps - 1) / kDecodeWarps;
+            unsigned long long page_at = 0;                  // of the cell j0 + lane
+            auto pages_of = [&](int j0) {
+                const int c = rq.first + c0 + warp + kDecodeWarps * (j0 + lane);
+                page_at = 0;
+                if (j0 + lane < count && c * kCellTokens < rq.length) {
+                    const uint32_t column = (uint32_t)c / p.page_cells;
+                    const int page = p.table[(long long)b * p.table_stride + column];
+                    if (page >= 0 && (uint32_t)page < p.pages)
+                        page_at = (unsigned long long)(p.cache + ((size_t)page * p.kv_heads + head) * p.page_bytes + (size_t)((uint32_t)c % p.page_cells) * CELL);
+                    else
+                        raise_error(p.err, kErrKv4Page);
+                }
+            };
+            auto issue = [&](int j) {
+                if (j < count) {
+                    if ((j & 31) == 0) pages_of(j);
+                    const unsigned long long at = __shfl_sync(0xffffffffu, page_at, j & 31);
+                    const uint32_t dst = ring_s + (uint32_t)(j % STAGES) * CELL;
+                    const uint8_t* src = at ? reinterpret_cast<const uint8_t*>(at) : p.cache;
+                    const uint32_t bytes = at ? 16u : 0u;
+#pragma unroll
+                    for (uint32_t i = 0; i < (CELL / 16 + 31) / 32; ++i) {
+                        const uint32_t o = (i * 32 + lane) * 16u;
+                        if (CELL % 512 == 0 || o < CELL) cp_async16(dst + o, src + (at ? o : 0), bytes);
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+#pragma unroll
+            for (int j = 0; j < STAGES - 1; ++j) issue(j);
+            for (int j = 0; j < count; ++j) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+                __syncwarp();
+                issue(j + STAGES - 1);                       // into the stage that the last step read
+                const uint8_t* st = ring + (size_t)(j % STAGES) * CELL;
+                const int tok0 = (rq.first + c0 + warp + kDecodeWarps * j) * kCellTokens;
+                const bool clear = tok0 >= clear_from && tok0 + kCellTokens <= clear_to;
+
+                // steps and offsets of the tokens gid, gid + 8
+                float ks[NG][2], ko[NG][2], vs[NG][2], vo[NG][2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bool inside = tok0 + gid + 8 * i < rq.length;      // behind the end lies what the page held before
+                    uint32_t a[NG], c[NG];
+                    load_words(a, st + kv4_key_step(D, GS, gid + 8 * i, 0));
+                    load_words(c, st + kv4_value_step(D, GS, gid + 8 * i, 0));
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        if (!inside) a[g] = c[g] = 0u;
+                        const float2 fa = unpack2<DT>(a[g]), fc = unpack2<DT>(c[g]);
+                        ks[g][i] = fa.x; ko[g][i] = fmaf(8.0f, fa.x, fa.y);
+                        vs[g][i] = fc.x; vo[g][i] = fmaf(8.0f, fc.x, fc.y);
+                    }
+                }
+                // ---- scores: rows = tokens gid, gid + 8; columns = queries 2 tig, 2 tig + 1
+                float s[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][i] = 0.0f;
+                constexpr int PER = NW < 4 ? NW : 4;          // words of a lane in a block
+                uint32_t xa[NW / PER][PER], xb[NW / PER][PER];
+#pragma unroll
+                for (int bl = 0; bl < NW / PER; ++bl) {
+                    load_words(xa[bl], st + ((bl * 16 + gid) * 4 + tig) * PER * 4);
+                    load_words(xb[bl], st + ((bl * 16 + gid + 8) * 4 + tig) * PER * 4);
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    float raw[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) raw[nt][i] = 0.0f;
+#pragma unroll
+                    for (int w = g * GS / 32; w < (g + 1) * GS / 32; ++w) {
+                        uint32_t ca[4], cb[4];
+                        code_pairs(xa[w / PER][w % PER], ca);
+                        code_pairs(xb[w / PER][w % PER], cb);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_16816<FP16>(raw[nt], ca[0], cb[0], ca[1], cb[1], qf[nt][w][0], qf[nt][w][1]);
+                            mma_16816<FP16>(raw[nt], ca[2], cb[2], ca[3], cb[3], qf[nt][w][2], qf[nt][w][3]);
+                        }
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            s[nt][i] = fmaf(raw[nt][i], ks[g][i >> 1], s[nt][i]);
+                            s[nt][i] = fmaf(ko[g][i >> 1], qs[nt][i & 1][g], s[nt][i]);
+                        }
+                }
+                bool follow = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[nt][i] *= sf[nt][i & 1];
+                        if (!clear) {
+                            const int tok = tok0 + gid + 8 * (i >> 1);
+                            if (tok < from[nt][i & 1] || tok >= to[nt][i & 1]) s[nt][i] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) follow |= fmaxf(s[nt][i], s[nt][2 + i]) > m[nt][i] + kGrow;
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) follow |= fmaxf(vs[g][0], vs[g][1]) * fv[g] > 2048.0f || fv[g] == 0.0f;
+                if (__any_sync(0xffffffffu, follow)) {
+                    // maxima over the cell, sums brought to them; rare once a few cells are done
+                    float down[NT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float top = fmaxf(s[nt][i], s[nt][2 + i]);
+#pragma unroll
+                            for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            top = fmaxf(top, m[nt][i]);
+                            down[nt][i] = top == m[nt][i] ? 1.0f : ex2(m[nt][i] - top);
+                            m[nt][i] = top;
+                            l[nt][i] *= down[nt][i];
+                        }
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs[g][0], vs[g][1])));
+                        int e = (int)(bits >> 23) - 127;               // the largest step is below 2^(e+1)
+                        e = max(e, -100);
+                        const float want = pow2(10 - min(e, 100));
+                        float by = 1.0f;
+                        if (fv[g] == 0.0f) fv[g] = want;
+                        else if (want < fv[g]) { by = want / fv[g]; fv[g] = want; }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const float d0 = by * down[nt][0], d1 = by * down[nt][1];
+                            off[nt][0][g] *= down[nt][0];
+                            off[nt][1][g] *= down[nt][1];
+#pragma unroll
+                            for (int i = g * GS / 16; i < (g + 1) * GS / 16; ++i) {
+                                acc[i][nt][0] *= d0; acc[i][nt][1] *= d1; acc[i][nt][2] *= d0; acc[i][nt][3] *= d1;
+                            }
+                        }
+                    }
+                }
+                float w[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // a row that has seen nothing yet has the maximum -inf: its weights are 0
+                        w[nt][i] = (!clear && s[nt][i] == -INFINITY) ? 0.0f : ex2(s[nt][i] - m[nt][i & 1]);
+                        l[nt][i & 1] += w[nt][i];
+                    }
+                // the lane's value codes: both planes (tokens 0..7, 8..15)
+                constexpr int VB = D < 128 ? 1 : D / 128, VP = NW / VB;      // blocks, words of a lane and plane in each
+                uint32_t xv[VB][2][VP];
+#pragma unroll
+                for (int bl = 0; bl < VB; ++bl)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) load_words(xv[bl][c], st + 8 * D + ((bl * 2 + c) * 32 + lane) * (VP * 4));
+                // ---- outputs: rows = elements, depth = tokens, columns = queries
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    uint32_t b0[NT], b1[NT];
+                    const float f0 = vs[g][0] * fv[g], f1 = vs[g][1] * fv[g];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        b0[nt] = movmatrix(half2_bits(w[nt][0] * f0, w[nt][1] * f0));
+                        b1[nt] = movmatrix(half2_bits(w[nt][2] * f1, w[nt][3] * f1));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if (clear) {
+                                off[nt][i][g] = fmaf(w[nt][i], vo[g][0], fmaf(w[nt][2 + i], vo[g][1], off[nt][i][g]));
+                            } else {                         // a token that this row does not see may hold no number
+                                off[nt][i][g] += w[nt][i] == 0.0f ? 0.0f : w[nt][i] * vo[g][0];
+                                off[nt][i][g] += w[nt][2 + i] == 0.0f ? 0.0f : w[nt][2 + i] * vo[g][1];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int i = g * GS / 32; i < (g + 1) * GS / 32; ++i) {      // elements 32 i .. + 31, four of them in the lane's word
+                        uint32_t c0v[4], c1v[4];
+                        code_pairs(xv[i / VP][0][i % VP], c0v);
+                        code_pairs(xv[i / VP][1][i % VP], c1v);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_16816<FP16>(acc[2 * i][nt], c0v[0], c0v[1], c1v[0], c1v[1], b0[nt], b1[nt]);
+                            mma_16816<FP16>(acc[2 * i + 1][nt], c0v[2], c0v[3], c1v[2], c1v[3], b0[nt], b1[nt]);
+                        }
+                    }
+                }
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
+
+            // ---- the warps' sums into shared memory
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int o = 4; o < 32; o *= 2) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], o);
+                    const int row = 8 * nt + 2 * tig + i;
+                    if (gid == 0) {
+                        merge_ml[(warp * Sh::kRows + row) * 2] = m[nt][i];
+                        merge_ml[(warp * Sh::kRows + row) * 2 + 1] = l[nt][i];
+                    }
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        float o4 = off[nt][i][g];
+#pragma unroll
+                        for (int o = 4; o < 32; o *= 2) o4 += __shfl_xor_sync(0xffffffffu, o4, o);
+                        const float unit = fv[g] != 0.0f ? 1.0f / fv[g] : 0.0f;
+#pragma unroll
+                        for (int k = g * GS / 32; k < (g + 1) * GS / 32; ++k) {
+                            float4 v;
+                            v.x = fmaf(acc[2 * k][nt][i], unit, o4);
+                            v.y = fmaf(acc[2 * k][nt][2 + i], unit, o4);
+                            v.z = fmaf(acc[2 * k + 1][nt][i], unit, o4);
+                            v.w = fmaf(acc[2 * k + 1][nt][2 + i], unit, o4);
+                            *reinterpret_cast<float4*>(merge + (size_t)(warp * Sh::kRows + row) * Sh::kRowStride + 32 * k + 4 * gid) = v;
+                        }
+                    }
+                }
+            __syncthreads();
+            const bool whole = c0 == 0 && c1 == rq.cells;
+            float* part = p.part + ((size_t)blockIdx.x * 2u + (c0 > 0 ? 0u : 1u)) * kv4_part_floats(D, NT);
+            for (int e = tid; e < Sh::kRows * (D / 4); e += kDecodeThreads) {
+                const int r = e / (D / 4), d4 = e % (D / 4);
+                float top = -INFINITY, mw[kDecodeWarps];
+#pragma unroll
+                for (int w = 0; w < kDecodeWarps; ++w) {
+                    mw[w] = merge_ml[(w * Sh::kRows + r) * 2];
+                    top = fmaxf(top, mw[w]);
+                }
+                float sum = 0.0f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kDecodeWarps; ++w) {
+                    if (mw[w] == -INFINITY && merge_ml[(w * Sh::kRows + r) * 2 + 1] == 0.0f) continue;       // saw nothing
+                    const float f = mw[w] == top ? 1.0f : ex2(mw[w] - top);
+                    const float4 o = *reinterpret_cast<const float4*>(merge + (size_t)(w * Sh::kRows + r) * Sh::kRowStride + 4 * d4);
+                    sum = fmaf(merge_ml[(w * Sh::kRows + r) * 2 + 1], f, sum);
+                    v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
+                }
+                const int row = row0 + r;
+                if (whole) {
+                    if (row < all_rows) {
+                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                        const long long tok = rq.start + row / (int)p.ratio, h = head * p.ratio + row % (int)p.ratio;
+                        T* dst = reinterpret_cast<T*>(p.out) + tok * p.out_token + h * p.out_head + 4 * d4;
+                        T o[4] = {Tr<DT>::from_f(v.x * inv), Tr<DT>::from_f(v.y * inv), Tr<DT>::from_f(v.z * inv), Tr<DT>::from_f(v.w * inv)};
+                        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+                        if (p.lse && d4 == 0) p.lse[(size_t)tok * p.kv_heads * p.ratio + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+                    }
+                } else {
+                    __stcg(reinterpret_cast<float4*>(part + r * D + 4 * d4), v);
+                    if (d4 == 0) {
+                        part[Sh::kRows * D + 2 * r] = top;
+                        part[Sh::kRows * D + 2 * r + 1] = sum;
+                    }
+                }
+            }
+            __syncthreads();
+            if (!whole && c0 == 0) {
+                // the segment ends in block (x + cells - 1) / per
+                cut.parts = (uint32_t)((x + rq.cells - 1) / per - blockIdx.x) + 1u;
+                cut.request = b; cut.row0 = (uint32_t)row0; cut.head = head; cut.start = (uint32_t)rq.start; cut.rows = (uint32_t)all_rows;
+            }
+            x += c1 - c0;
+            c0 = 0;
+            if (x < x1 && ++item == rq.tiles * (int)p.kv_heads) {
+                item = 0;
+                do rq = kv4_request(p, ++b, Sh::kRows, false); while (rq.tiles == 0);      // ends: cells remain
+            }
+        }
+    }
+    if (tid == 0) cuts[blockIdx.x] = cut;
+}
+
+// Adds the parts of a cut segment: one block per (block that began one, row of the tile).
+template <int D, int NT, int DT>
+__global__ void __launch_bounds__(128) kv4_join_kernel(Kv4Attn p, uint32_t blocks) {
+    using T = typename Tr<DT>::T;
+    constexpr int LANES = D / 4;                     // threads across a row
+    constexpr int WAYS = 128 / LANES;                // parts taken at the same time
+    __shared__ float4 s_v[WAYS][LANES];
+    __shared__ float s_ml[128][2];
+    __shared__ float s_all[2];
+    pdl_trigger();
+    pdl_wait();
+    const Kv4Cut cut = reinterpret_cast<const Kv4Cut*>(p.part + (size_t)blocks * 2u * kv4_part_floats(D, NT))[blockIdx.x];
+    const uint32_t r = blockIdx.y, row = cut.row0 + r;
+    if (cut.parts == 0 || row >= cut.rows) return;
+    const float* base = p.part + (size_t)blockIdx.x * 2u * kv4_part_floats(D, NT);
+    // part 0 is this block's second, part i the first of block + i
+    auto part = [&](uint32_t i) { return base + (size_t)(i == 0 ? 1u : 2u * i) * kv4_part_floats(D, NT); };
+    const uint32_t tid = threadIdx.x;
+    float m = -INFINITY, l = 0.0f;
+    for (uint32_t i = tid; i < cut.parts; i += 128u) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(i) + 8 * NT * D + 2 * r));
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;
+        const float top = fmaxf(m, ml.x);
+        l = l * (m == top ? 1.0f : ex2(m - top)) + ml.y * (ml.x == top ? 1.0f : ex2(ml.x - top));
+        m = top;
+    }
+    s_ml[tid][0] = m;
+    s_ml[tid][1] = l;
+    __syncthreads();
+    if (tid < 32) {
+        for (int i = 1; i < 4; ++i) {
+            const float m2 = s_ml[tid + 32 * i][0], top = fmaxf(m, m2);
+            l = l * (m == top ? 1.0f : ex2(m - top)) + s_ml[tid + 32 * i][1] * (m2 == top ? 1.0f : ex2(m2 - top));
+            m = top;
+        }
+#pragma unroll
+        for (int o = 16; o; o /= 2) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o), top = fmaxf(m, m2);
+            l = l * (m == top ? 1.0f : ex2(m - top)) + l2 * (m2 == top ? 1.0f : ex2(m2 - top));
+            m = top;
+        }
+        if (tid == 0) { s_all[0] = m; s_all[1] = l; }
+    }
+    __syncthreads();
+    const float top = s_all[0], sum = s_all[1];
+    const uint32_t way = tid / LANES, d4 = tid % LANES;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (uint32_t i = way; i < cut.parts; i += WAYS) {
+        const float* at = part(i);
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(at + 8 * NT * D + 2 * r));
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(at + r * D + 4 * d4));
+        const float f = (ml.x == -INFINITY && ml.y == 0.0f) ? 0.0f : ml.x == top ? 1.0f : ex2(ml.x - top);
+        v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
+    }
+    s_v[way][d4] = v;
+    __syncthreads();
+    if (way == 0) {
+#pragma unroll
+        for (int w = 1; w < WAYS; ++w) {
+            const float4 o = s_v[w][d4];
+            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const long long tok = cut.start + row / p.ratio, h = cut.head * p.ratio + row % p.ratio;
+        T* dst = reinterpret_cast<T*>(p.out) + tok * p.out_token + h * p.out_head + 4 * d4;
+        T o[4] = {Tr<DT>::from_f(v.x * inv), Tr<DT>::from_f(v.y * inv), Tr<DT>::from_f(v.z * inv), Tr<DT>::from_f(v.w * inv)};
+        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+        if (p.lse && d4 == 0) p.lse[(size_t)tok * p.kv_heads * p.ratio + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+    }
+}
+
+// ---- launch, one translation unit per head size ------------------------------------------------------------
+template <int D, int GS, int NT, int DT> int decode_blocks_per_sm() {
+    static int per_sm[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (!per_sm[dev]) {
+        const size_t smem = decode_smem<D, GS, NT>();
+        int n = 0;
+        if (cudaFuncSetAttribute(kv4_decode_kernel<D, GS, NT, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_decode_kernel<D, GS, NT, DT>, kDecodeThreads, smem) != cudaSuccess || n < 1)
+            return 0;
+        per_sm[dev] = n;
+    }
+    return per_sm[dev];
+}
+
+template <int D, int GS, int NT, int DT> cudaError_t run_decode(const Kv4Attn& p, uint32_t blocks, cudaStream_t s) {
+    if (!decode_blocks_per_sm<D, GS, NT, DT>()) return cudaErrorInvalidConfiguration;
+    kv4_decode_kernel<D, GS, NT, DT><<<blocks, kDecodeThreads, decode_smem<D, GS, NT>(), s>>>(p);
+    if (cudaError_t e = cudaGetLastError()) return e;
+    kv4_join_kernel<D, NT, DT><<<dim3(blocks, 8 * NT), 128, 0, s>>>(p, blocks);
+    return cudaGetLastError();
+}
+
+// f<GS, NT, DT>() of a head size
+template <int D, typename F> auto for_decode(uint32_t group, uint32_t nt, int dt, F&& f) -> decltype(f.template operator()<32, 1, FP16>()) {
+#define KV4_CASE(G_, N_)                                                                                                             \
+    if constexpr (G_ <= D && (N_ == 1 || D <= 128))                                                                                  \
+        if (group == G_ && nt == N_) return dt == FP16 ? f.template operator()<G_, N_, FP16>() : f.template operator()<G_, N_, BF16>()
+    KV4_CASE(32, 1);
+    KV4_CASE(64, 1);
+    KV4_CASE(128, 1);
+    KV4_CASE(32, 2);
+    KV4_CASE(64, 2);
+    KV4_CASE(128, 2);
+#undef KV4_CASE
+    return f.none();
+}
+
+template <int D> struct BlocksCall {
+    int none() { return 0; }
+    template <int GS, int NT, int DT> int operator()() { return decode_blocks_per_sm<D, GS, NT, DT>(); }
+};
+template <int D> struct DecodeCall {
+    const Kv4Attn& p;
+    uint32_t blocks;
+    cudaStream_t s;
+    cudaError_t none() { return cudaErrorInvalidValue; }
+    template <int GS, int NT, int DT> cudaError_t operator()() { return run_decode<D, GS, NT, DT>(p, blocks, s); }
+};
+
+}  // namespace dd

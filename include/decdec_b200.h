@@ -63,7 +63,9 @@ int decdec_compiled_arch(void);
 /* ---- device-side failures.  NO COUNTERPART IN THE REFERENCE (it ignores launch and device errors,
  * dec_config.cu:204-208).  Every wait inside the kernels of this library is bounded; a thread block that gives up
  * stores a code into the error word of the (device, stream) workspace: 1 = a wait for a shared-memory stage ran
- * out (DECDEC_PIPE_WAIT_NS, default 50 ms), 2 = the launch did not get the shared-memory layout it was sized for.
+ * out (DECDEC_PIPE_WAIT_NS, default 50 ms), 2 = the launch did not get the shared-memory layout it was sized for,
+ * 3 = a call on the 4-bit key/value cache met a page or a slot outside the cache, or a length beyond its block table (it reads zeros there
+ * and writes nothing).
  * The output of that launch is then incomplete.  The word lives in mapped host memory, so every later compute call
  * on that stream sees it without a copy and fails with DECDEC_E_DEVICE until the stream is reset.
  *   decdec_stream_status  *error_out = the word (0 = fine); does not synchronise.
@@ -188,6 +190,65 @@ int decdec_dummy_lutgemm(const void* x_dev, void* y_dev, const int32_t* qweight,
                          long long dummy_iters, void* stream);
 int decdec_dummy_sqllm(const void* x_dev, void* y_dev, const int32_t* qweight, const void* lut,
                        uint32_t N, uint32_t K, int bitwidth, int dtype, int dummy_sm, long long dummy_iters, void* stream);
+
+/* ---- the 4-bit key/value cache and what stands around it.  NO COUNTERPART IN THE REFERENCE BINDING (its models keep a dense
+ * 16-bit cache, end-to-end/model.py).
+ *
+ * The cache is uint8 [pages, kv_heads, bytes of a page], 16-byte aligned; a page of `page_size` tokens (a multiple of 16) is a run of
+ * cells of 16 tokens.  A cell of a head of `head_dim` D (64, 128, 256) elements with `group_size` G (32, 64, 128, not above D) is
+ * 16 (D + 8 D/G) bytes:
+ *   key codes    8 D bytes    [D/128][token][4][word of 32][2] 16-bit words of four codes; element = 128 b + 32 w + 8 [4] + 4 [2] + code
+ *   value codes  8 D bytes    [D/128][token/8][8][token%8/2][word of 64][2][token%2]; element = 128 b + 64 w + 32 [2] + 4 [8] + code
+ *   key steps    64 D/G bytes [token][group] pairs (step, offset) of dtype
+ *   value steps  64 D/G bytes the same
+ * (a head of 64 is one block of two words of 32, one of 64).  An element is offset + step * code; append takes offset = least element of
+ * the group, step = (largest - least) / 15 rounded to dtype, code = (x - offset) / step to the nearest, ties to even.  A group with an
+ * infinity or a NaN reads back as NaN.  dtype is DECDEC_FP16 or DECDEC_BF16 except in decdec_rotary, which takes all three.
+ *
+ * Rows are [tokens][heads][head_dim] with strides in elements between tokens and heads; elements of a head are neighbours.  `*_wide`: 1 if
+ * the integers are int64, 0 if int32.  A slot is page * page_size + place; a negative slot is skipped (gather: zeros).  Two rows of one
+ * append must not share a slot.  A page or slot outside the cache, or a length beyond the block table, raises error 3 of the stream.
+ *
+ *   decdec_rotary       (a, b) -> ((a cos - b sin) factor, (b cos + a sin) factor) with the angle position * frequencies[i] (64 bits), for
+ *                       the pairs i of the first `rotary_dim` elements: neighbours if `interleaved`, else rotary_dim/2 apart.  The rest is
+ *                       copied.  Outputs may be the inputs themselves (same pointer and strides), not overlap them otherwise.
+ *   decdec_kv4_plan     lengths[requests] tokens held, fresh[requests] tokens to come, table [requests][table_cols] of pages, free_pages with
+ *                       free_count[0] pages left, the last taken first.  Gives each request the pages that it lacks (in order of requests,
+ *                       entered in `table`), positions and slots of the new tokens one request after another (tokens entries; behind the
+ *                       last: position 0, slot -1), query_starts[requests + 1], out_lengths, out_free_count[1] and status[1]: 0, or a sum
+ *                       of 1 = too few free pages, 2 = a request is longer than its table row, 4 = more than `tokens` new tokens,
+ *                       8 = a negative count; then nothing is given: slots -1, query_starts 0, lengths and free_count as they were.
+ *                       Outputs must not overlap inputs.
+ *   decdec_kv4_append   writes rows of keys and values to their slots.
+ *   decdec_kv4_gather   reads them: contiguous [tokens][kv_heads][head_dim], offset + step * code rounded to dtype (and kept finite).
+ *   decdec_kv4_attention  out = softmax(scale q k^T) v per query head (head h reads key head h / (heads / kv_heads)).  Request b has the
+ *                       rows query_starts[b] .. query_starts[b+1] - 1 and lengths[b] tokens in the cache, its own among them: row i stands
+ *                       at position lengths[b] - queries + i and sees the tokens up to its own, the last `window` of them if window > 0.  A
+ *                       row that sees nothing gives zeros (lse -inf).  max_queries bounds the rows of a request and chooses the kernel;
+ *                       requests with more are computed all the same.  Rows behind the last request stay as they are, or are cleared if
+ *                       clear_tail.  lse, if not null: fp32 [rows][heads], the logarithm of the sum of exp(scaled scores).
+ *                       The workspace (bytes from _workspace, 16-byte aligned) holds nothing between calls; calls that may overlap in time
+ *                       need one each. */
+int decdec_rotary(const void* q, int64_t q_token, int64_t q_head, uint32_t q_heads, const void* k, int64_t k_token, int64_t k_head, uint32_t k_heads,
+                  void* q_out, int64_t qo_token, int64_t qo_head, void* k_out, int64_t ko_token, int64_t ko_head, const void* positions,
+                  int positions_wide, const double* frequencies, uint32_t tokens, uint32_t head_dim, uint32_t rotary_dim, int interleaved,
+                  float factor, int dtype, void* stream);
+int decdec_kv4_plan(const int32_t* lengths, const int32_t* fresh, uint32_t requests, int32_t* table, int64_t table_stride, uint32_t table_cols,
+                    const int32_t* free_pages, uint32_t free_capacity, const int32_t* free_count, uint32_t page_size, uint32_t tokens,
+                    int64_t* positions, int64_t* slots, int32_t* query_starts, int32_t* out_lengths, int32_t* out_free_count, int32_t* status,
+                    void* stream);
+int decdec_kv4_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* slots, int slots_wide,
+                      uint32_t tokens, void* cache, uint32_t pages, uint32_t page_size, uint32_t kv_heads, uint32_t head_dim, uint32_t group_size,
+                      int dtype, void* stream);
+int decdec_kv4_gather(const void* cache, uint32_t pages, uint32_t page_size, uint32_t kv_heads, uint32_t head_dim, uint32_t group_size,
+                      const void* slots, int slots_wide, uint32_t tokens, void* k_out, void* v_out, int dtype, void* stream);
+int decdec_kv4_attention_workspace(uint32_t requests, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t group_size,
+                                   uint32_t max_queries, int dtype, size_t* bytes);
+int decdec_kv4_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t out_token, int64_t out_head, float* lse, const void* cache,
+                         uint32_t pages, uint32_t page_size, const int32_t* table, int64_t table_stride, uint32_t table_cols, const int32_t* lengths,
+                         const int32_t* query_starts, uint32_t requests, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                         uint32_t group_size, uint32_t max_queries, float scale, uint32_t window, int clear_tail, void* workspace,
+                         size_t workspace_bytes, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
