@@ -67,13 +67,19 @@ def build_lib(verbose: bool = False, force: bool = False) -> Path:
 
 
 def build_shim(force: bool = False) -> Path:
-    """decdec_ext: pybind11/torch module with the reference's 17 functions (bindings.cpp:17-41)."""
+    """decdec_ext: pybind11/torch module with the reference's 17 functions (bindings.cpp:17-41); and _kv4, behind decdec_b200.kv4."""
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        out, _ = ex.map(lambda a: _build_torch_module(*a, force), [("decdec_ext", "shim.cpp"), ("_kv4", "shim_kv4.cpp")])
+    return out
+
+
+def _build_torch_module(name: str, source: str, force: bool) -> Path:
     import torch
     from torch.utils import cpp_extension
 
     suffix = sysconfig.get_config_var("EXT_SUFFIX")
-    out = PKG / f"decdec_ext{suffix}"
-    src = CSRC / "shim.cpp"
+    out = PKG / f"{name}{suffix}"
+    src = CSRC / source
     if not force and not _stale(out, [src, PKG.parent / "include" / "decdec_b200.h"]):
         return out
     inc = cpp_extension.include_paths(device_type="cuda") if hasattr(cpp_extension, "include_paths") else []
@@ -82,7 +88,7 @@ def build_shim(force: bool = False) -> Path:
     except TypeError:
         inc = cpp_extension.include_paths(cuda=True)
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=decdec_ext",
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-DTORCH_EXTENSION_NAME={name}",
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{p}" for p in inc], f"-I{sysconfig.get_paths()['include']}", f"-I{PKG.parent / 'include'}",
            str(src), "-o", str(out), f"-L{PKG}", "-ldecdec_b200", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu",

@@ -16,16 +16,13 @@ format.  Tensors: fp16 or bf16, [tokens, heads, head_dim], any strides with neig
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 from typing import NamedTuple, Optional
 
 import torch
 
-from . import capi
-from .ops import _DT, _call, _check, _stream
-
-_INTS = (torch.int32, torch.int64)
+from . import _kv4
+from .ops import _check
 
 
 class Plan(NamedTuple):
@@ -39,53 +36,13 @@ class Plan(NamedTuple):
 
 def cell_bytes(head_dim: int, group_size: int) -> int:
     """Bytes of 16 tokens of one head."""
-    _check(head_dim in (64, 128, 256), f"head_dim must be 64, 128 or 256, got {head_dim}.")
-    _check(group_size in (32, 64, 128) and group_size <= head_dim, f"group_size must be 32, 64 or 128 and not above head_dim, got {group_size}.")
-    return 16 * (head_dim + 8 * head_dim // group_size)
+    return _kv4.cell_bytes(head_dim, group_size)
 
 
 def empty_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, group_size: int, device="cuda") -> torch.Tensor:
     """A cache of `pages` pages of `page_size` tokens (a multiple of 16): uint8 [pages, kv_heads, bytes of a page], zeros."""
     _check(page_size > 0 and page_size % 16 == 0, f"page_size must be a multiple of 16, got {page_size}.")
     return torch.zeros((pages, kv_heads, page_size // 16 * cell_bytes(head_dim, group_size)), dtype=torch.uint8, device=device)
-
-
-def _cache(cache: torch.Tensor, head_dim: int, group_size: int):
-    """pages, page_size, kv_heads of a cache."""
-    _check(cache.dtype == torch.uint8 and cache.dim() == 3 and cache.is_contiguous(), "cache must be a contiguous uint8 tensor [pages, kv_heads, bytes].")
-    pages, kv_heads, size = cache.shape
-    cell = cell_bytes(head_dim, group_size)
-    _check(size > 0 and size % cell == 0, f"a page of {size} bytes is no whole number of cells of {cell} bytes (head_dim {head_dim}, group_size {group_size}).")
-    return pages, size // cell * 16, kv_heads
-
-
-def _rows(t: torch.Tensor, name: str) -> tuple:
-    _check(t.dim() == 3, f"{name} must be of shape (tokens, heads, head_dim).")
-    _check(t.stride(2) == 1 or t.size(2) <= 1, f"elements of a head of {name} must be neighbours.")
-    return t.data_ptr(), t.stride(0), t.stride(1)
-
-
-def _same_device(first: torch.Tensor, *others) -> None:
-    _check(first.is_cuda, "tensors must be on GPU.")
-    for t in others:
-        _check(t is None or t.device == first.device, "all tensors must be on the same GPU.")
-
-
-def _index(t: torch.Tensor, n: int, name: str) -> tuple:
-    _check(t.dtype in _INTS and t.dim() == 1 and t.is_contiguous() and t.numel() == n, f"{name} must be a contiguous int32 or int64 tensor of {n} entries.")
-    return t.data_ptr(), int(t.dtype == torch.int64)
-
-
-def _int32(t: torch.Tensor, n: Optional[int], name: str) -> int:
-    _check(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and (n is None or t.numel() == n),
-           f"{name} must be a contiguous int32 tensor" + ("." if n is None else f" of {n} entries."))
-    return t.data_ptr()
-
-
-def _table(t: torch.Tensor, requests: int) -> tuple:
-    _check(t.dtype == torch.int32 and t.dim() == 2 and t.size(0) == requests and (t.size(1) <= 1 or t.stride(1) == 1),
-           "block_table must be an int32 tensor of shape (requests, pages) with neighbouring entries.")
-    return t.data_ptr(), t.stride(0), t.size(1)
 
 
 # ---- rotary positions ---------------------------------------------------------------------------------------
@@ -134,32 +91,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     """Positions into queries and keys (k may be None): the first 2 * len(frequencies) elements of each head are turned, the rest copied.
     Pairs are neighbours if `interleaved`, else half of the turned elements apart.  Angles are taken in 64 bits.  fp16, bf16, fp32.
     out=(q', k'): where to, which may be q and k themselves.  Returns (q', k')."""
-    _check(q.dtype in _DT, "Unsupported data type.")
-    tokens, heads, d = q.shape if q.dim() == 3 else (0, 0, 0)
-    args = [*_rows(q, "q"), heads]
-    _same_device(q, k, positions, frequencies)
-    if k is not None:
-        args += [*_rows(k, "k"), k.size(1)]
-        _check(k.dtype == q.dtype and k.size(0) == tokens and k.size(2) == d, "q and k must share data type, tokens and head_dim.")
-    else:
-        args += [None, 0, 0, 0]
-    _check(frequencies.dtype == torch.float64 and frequencies.dim() == 1 and frequencies.is_contiguous(), "frequencies must be a contiguous float64 vector.")
-    _check(0 < 2 * frequencies.numel() <= d, "there are more frequencies than pairs in a head, or none.")
-    at, wide = _index(positions, tokens, "positions")
-    if out is None:
-        q_out = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty((tokens, k.size(1), d), dtype=q.dtype, device=q.device)
-    else:
-        q_out, k_out = out
-        _check(q_out.shape == q.shape and q_out.dtype == q.dtype and (k is None) == (k_out is None), "out must have the shapes and types of q and k.")
-        _check(k is None or (k_out.shape == k.shape and k_out.dtype == k.dtype), "out must have the shapes and types of q and k.")
-        _same_device(q, q_out, k_out)
-    args += _rows(q_out, "out")
-    args += [None, 0, 0] if k is None else _rows(k_out, "out")
-    with torch.cuda.device(q.device):
-        _call("decdec_rotary", *args, at, wide, frequencies.data_ptr(), tokens, d, 2 * frequencies.numel(), int(interleaved), float(factor),
-              _DT[q.dtype], _stream())
-    return q_out, k_out
+    return _kv4.rotary(q, k, positions, frequencies, interleaved, factor, *((None, None) if out is None else out))
 
 
 # ---- pages and slots of a step ---------------------------------------------------------------------------------
@@ -171,19 +103,7 @@ def plan(lengths: torch.Tensor, new_lengths: torch.Tensor, block_table: torch.Te
     A request that outgrows its pages takes the last of free_pages[:free_count]; they are entered in `block_table`, which is
     written in place.  `tokens`: entries of positions and slots, at least the sum of new_lengths.  All or nothing: if status is not 0
     no page is given, slots are -1, query_starts 0, lengths and free_count as they were."""
-    requests = lengths.numel()
-    _same_device(lengths, new_lengths, block_table, free_pages, free_count)
-    device = lengths.device
-    args = [_int32(lengths, None, "lengths"), _int32(new_lengths, requests, "new_lengths"), requests, *_table(block_table, requests),
-            _int32(free_pages, None, "free_pages"), free_pages.numel(), _int32(free_count, 1, "free_count"), int(page_size), int(tokens)]
-    _check(tokens >= 0, "tokens must not be negative.")
-    wide = torch.empty((2, tokens), dtype=torch.int64, device=device)
-    narrow = torch.empty(2 * requests + 3, dtype=torch.int32, device=device)
-    starts, after, left, status = narrow.split([requests + 1, requests, 1, 1])
-    with torch.cuda.device(device):
-        _call("decdec_kv4_plan", *args, wide[0].data_ptr(), wide[1].data_ptr(), starts.data_ptr(), after.data_ptr(), left.data_ptr(), status.data_ptr(),
-              _stream())
-    return Plan(wide[0], wide[1], starts, after, left, status)
+    return Plan(*_kv4.plan(lengths, new_lengths, block_table, free_pages, free_count, page_size, tokens))
 
 
 # ---- rows into the cache and out of it ---------------------------------------------------------------------------
@@ -191,30 +111,12 @@ def plan(lengths: torch.Tensor, new_lengths: torch.Tensor, block_table: torch.Te
 def append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, group_size: int) -> None:
     """Writes rows of keys and values [tokens, kv_heads, head_dim] to their slots (page * page_size + place; negative: skipped).
     Slots must differ: of two rows with the same slot any mixture may stay."""
-    _check(k.dtype in (torch.float16, torch.bfloat16) and v.dtype == k.dtype, "k and v must both be half or both bfloat16.")
-    args = [*_rows(k, "k"), *_rows(v, "v")]
-    _check(k.shape == v.shape, "k and v must have the same shape.")
-    _same_device(k, v, slots, cache)
-    pages, page_size, kv_heads = _cache(cache, k.size(2), group_size)
-    _check(k.size(1) == kv_heads, f"the cache has {kv_heads} heads, k and v have {k.size(1)}.")
-    at, wide = _index(slots, k.size(0), "slots")
-    with torch.cuda.device(k.device):
-        _call("decdec_kv4_append", *args, at, wide, k.size(0), cache.data_ptr(), pages, page_size, kv_heads, k.size(2), group_size, _DT[k.dtype], _stream())
+    _kv4.append(cache, k, v, slots, group_size)
 
 
 def gather(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, group_size: int, dtype: torch.dtype) -> tuple:
     """Dense keys and values [len(slots), kv_heads, head_dim] of slots, in any order; zeros for negative ones."""
-    _check(dtype in (torch.float16, torch.bfloat16), "dtype must be half or bfloat16.")
-    _same_device(cache, slots)
-    pages, page_size, kv_heads = _cache(cache, head_dim, group_size)
-    n = slots.numel()
-    at, wide = _index(slots, n, "slots")
-    out = torch.empty((2, n, kv_heads, head_dim), dtype=dtype, device=cache.device)
-    k, v = out[0], out[1]
-    with torch.cuda.device(cache.device):
-        _call("decdec_kv4_gather", cache.data_ptr(), pages, page_size, kv_heads, head_dim, group_size, at, wide, n, k.data_ptr(), v.data_ptr(), _DT[dtype],
-              _stream())
-    return k, v
+    return _kv4.gather(cache, slots, head_dim, group_size, dtype)
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------
@@ -228,31 +130,5 @@ def attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, l
     window > 0: each row sees the last `window` tokens up to its own.  A row that sees no token gives zeros.  max_queries: the most rows of a
     request (default: all rows), which chooses the kernel.  scale: default head_dim ** -0.5.  Rows behind the last request are left as
     they are in `out`, zeros where `out` is not given.  return_lse: also the fp32 logarithms [tokens, heads] of the sums of exp(scale q k^T)."""
-    _check(q.dtype in (torch.float16, torch.bfloat16), "q must be half or bfloat16.")
-    at = _rows(q, "q")
-    tokens, heads, d = q.shape
-    _same_device(q, cache, block_table, lengths, query_starts, out)
-    pages, page_size, kv_heads = _cache(cache, d, group_size)
-    _check(kv_heads > 0 and heads > 0 and heads % kv_heads == 0, f"heads of q must be a multiple of the cache's {kv_heads}, got {heads}.")
-    requests = lengths.numel()
-    table = _table(block_table, requests)
-    lens, starts = _int32(lengths, None, "lengths"), _int32(query_starts, requests + 1, "query_starts")
-    _check(window >= 0, "window must not be negative.")
-    _check(max_queries is None or max_queries >= 1, "max_queries must be at least 1.")
-    max_queries = max(1, tokens if max_queries is None else min(int(max_queries), tokens))
-    scale = d ** -0.5 if scale is None else float(scale)
-    given = out is not None
-    if given:
-        _check(out.shape == q.shape and out.dtype == q.dtype, "out must have the shape and type of q.")
-    else:
-        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
-    lse = torch.full((tokens, heads), -math.inf, dtype=torch.float32, device=q.device) if return_lse else None
-    dt = _DT[q.dtype]
-    with torch.cuda.device(q.device):
-        size = C.c_size_t(0)
-        _call("decdec_kv4_attention_workspace", requests, tokens, heads, kv_heads, d, group_size, max_queries, dt, C.byref(size))
-        workspace = torch.empty(size.value, dtype=torch.uint8, device=q.device)
-        _call("decdec_kv4_attention", *at, *_rows(out, "out"), lse.data_ptr() if return_lse else None, cache.data_ptr(), pages, page_size, *table, lens, starts,
-              requests, tokens, heads, kv_heads, d, group_size, max_queries, scale, min(int(window), 0x7fffffff), int(not given), workspace.data_ptr(),
-              workspace.numel(), dt, _stream())
+    out, lse = _kv4.attention(q, cache, block_table, lengths, query_starts, group_size, max_queries, scale, window, out, return_lse)
     return (out, lse) if return_lse else out
