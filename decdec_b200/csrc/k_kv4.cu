@@ -70,9 +70,8 @@ template <int DT, bool HALF>
 cudaError_t rotary_any(int vec, dim3 grid, cudaStream_t s, const Rows& q, uint32_t qh, const Rows& k, uint32_t kh, const Rows& qo, const Rows& ko,
                        const void* positions, int wide, const double* f, uint32_t tokens, uint32_t d, uint32_t r, float factor) {
     constexpr int W = DT == FP32 ? 4 : 8;
-    if (vec) rotary_kernel<DT, HALF, W><<<grid, 256, 0, s>>>(q, qh, k, kh, qo, ko, positions, wide, f, tokens, d, r, factor);
-    else rotary_kernel<DT, HALF, 1><<<grid, 256, 0, s>>>(q, qh, k, kh, qo, ko, positions, wide, f, tokens, d, r, factor);
-    return cudaGetLastError();
+    return launch_early(vec ? rotary_kernel<DT, HALF, W> : rotary_kernel<DT, HALF, 1>, grid, dim3(256), 0, s, q, qh, k, kh, qo, ko, positions, wide, f, tokens, d, r,
+                        factor);
 }
 
 // ---- plan of a step --------------------------------------------------------------------------------------
@@ -342,9 +341,8 @@ cudaError_t run_append(const Rows& k, const Rows& v, const void* slots, int wide
     uint64_t blocks = (units + per_block - 1) / per_block;
     const uint64_t most = (uint64_t)device_sms() * 8u;
     if (blocks > most) blocks = most;
-    if (vec) append_kernel<DT, D, GS, true><<<(unsigned)blocks, 256, 0, s>>>(k, v, slots, wide, c, tokens, err);
-    else append_kernel<DT, D, GS, false><<<(unsigned)blocks, 256, 0, s>>>(k, v, slots, wide, c, tokens, err);
-    return cudaGetLastError();
+    return launch_early(vec ? append_kernel<DT, D, GS, true> : append_kernel<DT, D, GS, false>, dim3((unsigned)blocks), dim3(256), 0, s, k, v, slots, wide, c,
+                        tokens, err);
 }
 
 template <int DT, int D, int GS>
@@ -352,8 +350,7 @@ cudaError_t run_gather(const Kv4Cache& c, const void* slots, int wide, void* k, 
     uint64_t blocks = ((uint64_t)tokens * c.kv_heads * (D / 4) + 255u) / 256u;
     const uint64_t most = (uint64_t)device_sms() * 16u;
     if (blocks > most) blocks = most;
-    gather_kernel<DT, D, GS><<<(unsigned)blocks, 256, 0, s>>>(c, slots, wide, k, v, tokens, err);
-    return cudaGetLastError();
+    return launch_early(gather_kernel<DT, D, GS>, dim3((unsigned)blocks), dim3(256), 0, s, c, slots, wide, k, v, tokens, err);
 }
 
 // f.template operator()<DT, D, GS>() for the types, heads and groups that the cache takes
@@ -496,8 +493,7 @@ int decdec_kv4_plan(const int32_t* lengths, const int32_t* fresh, uint32_t reque
     uint32_t blocks = (tokens + kPlanThreads - 1u) / kPlanThreads;
     if (blocks == 0) blocks = 1;
     if (blocks > device_sms()) blocks = device_sms();
-    plan_kernel<<<blocks, kPlanThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
-    return launched(cudaGetLastError(), "plan launch");
+    return launched(launch_early(plan_kernel, dim3(blocks), dim3(kPlanThreads), 0, reinterpret_cast<cudaStream_t>(stream), p), "plan launch");
 }
 
 int decdec_kv4_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* slots, int slots_wide,

@@ -12,6 +12,9 @@
 #pragma once
 #include "common.cuh"
 
+#include <cstdlib>
+#include <utility>
+
 namespace dd {
 
 constexpr int kCellTokens = 16;
@@ -83,6 +86,27 @@ KV4_DECODE(64);
 KV4_DECODE(128);
 KV4_DECODE(256);
 #undef KV4_DECODE
+
+// A launch whose blocks may become resident while the previous kernel of the stream drains (every kernel here waits for it before
+// it reads anything); DECDEC_PDL=0 turns that off.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args&&... args) {
+    static const bool early = [] {
+        const char* v = getenv("DECDEC_PDL");
+        return !(v && v[0] == '0');
+    }();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
 
 int stream_error_word(cudaStream_t s, unsigned** err);    // 0, or the code that the call has to return
 

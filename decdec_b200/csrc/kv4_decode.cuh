@@ -23,10 +23,13 @@
 #pragma once
 #include "kv4.cuh"
 
+#include <type_traits>
+
 namespace dd {
 
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeWarps = 4;
+constexpr uint32_t kNoCell = 0xffffffffu;
 constexpr float kGrow = 4.0f;          // a running maximum follows once it is 2^4 behind
 
 // one part of a cut segment: [rows of a tile][D] sums, then [rows][2] maximum (log2 units) and sum
@@ -65,7 +68,8 @@ __device__ __forceinline__ void code_pairs(uint32_t x, uint32_t (&h)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t y = i < 2 ? x : x >> 8;
-        const uint32_t m = (y & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+        uint32_t m;                                          // (y & mask) | 0x64006400 as one instruction
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(y), "r"(i & 1 ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
         const __half2 v = *reinterpret_cast<const __half2*>(&m);
         const __half2 r = i & 1 ? __hfma2(v, by, high) : __hadd2(v, low);
         h[i] = *reinterpret_cast<const uint32_t*>(&r);
@@ -117,9 +121,12 @@ template <int D, int NT> struct DecodeShape {
     static constexpr int kRowStride = D + 4;            // floats; keeps the warps' 16-byte stores apart by banks
     static constexpr int kMergeFloats = kDecodeWarps * kRows * (kRowStride + 2);
 };
-template <int D, int GS> __host__ __device__ constexpr int decode_stages() { return kv4_cell_bytes(D, GS) > 2600 ? 3 : 4; }
+// A step of a warp is two neighbouring cells (32 tokens), and kStages steps of a warp lie in shared memory.  The warps' sums are added in
+// the same memory once a segment's steps are through.
+constexpr int kStages = 3;
 template <int D, int GS, int NT> __host__ __device__ constexpr size_t decode_smem() {
-    return (size_t)kDecodeWarps * decode_stages<D, GS>() * kv4_cell_bytes(D, GS) + DecodeShape<D, NT>::kMergeFloats * 4u;
+    const size_t ring = (size_t)kDecodeWarps * kStages * 2u * kv4_cell_bytes(D, GS), merge = DecodeShape<D, NT>::kMergeFloats * 4u;
+    return ring > merge ? ring : merge;
 }
 
 template <int D, int GS, int NT, int DT>
@@ -128,7 +135,6 @@ __global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
     using Sh = DecodeShape<D, NT>;
     constexpr int NG = D / GS;                  // groups of a head
     constexpr int NW = D / 32;                  // words of 32 elements
-    constexpr int STAGES = decode_stages<D, GS>();
     constexpr uint32_t CELL = kv4_cell_bytes(D, GS);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long s_sum[kDecodeThreads / 32];
@@ -137,9 +143,9 @@ __global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gid = lane >> 2, tig = lane & 3;
-    uint8_t* ring = smem + (size_t)warp * STAGES * CELL;
+    uint8_t* ring = smem + (size_t)warp * kStages * 2 * CELL;
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-    float* merge = reinterpret_cast<float*>(smem + (size_t)kDecodeWarps * STAGES * CELL);     // [warp][row][kRowStride]
+    float* merge = reinterpret_cast<float*>(smem);                                            // [warp][row][kRowStride]
     float* merge_ml = merge + kDecodeWarps * Sh::kRows * Sh::kRowStride;                      // [warp][row][2]
     uint8_t* after = reinterpret_cast<uint8_t*>(p.part + (size_t)gridDim.x * 2u * kv4_part_floats(D, NT));
     Kv4Cut* cuts = reinterpret_cast<Kv4Cut*>(after);
@@ -278,21 +284,22 @@ __global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
             }
             // tokens that each of this lane's rows sees: [from, to)
             int from[NT][2], to[NT][2];
-            const int pos0 = rq.length - rq.queries;
+            const int pos0 = rq.length - rq.queries, end = (rq.first + c1) * kCellTokens;      // the segment's cells end there
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int row = row0 + 8 * nt + 2 * tig + i;
                     const int pos = pos0 + min(row, all_rows - 1) / (int)p.ratio;
-                    to[nt][i] = max(pos + 1, 0);
+                    to[nt][i] = min(max(pos + 1, 0), end);
                     from[nt][i] = p.window ? (int)max(0ll, (long long)pos - (long long)p.window + 1) : 0;
                 }
             // cells between these are seen whole by every row of the tile
             const int first_pos = pos0 + row0 / (int)p.ratio, last_pos = pos0 + (min(row0 + Sh::kRows, all_rows) - 1) / (int)p.ratio;
-            const int clear_to = max(first_pos + 1, 0), clear_from = p.window ? (int)max(0ll, (long long)last_pos - (long long)p.window + 1) : 0;
+            const int clear_to = min(max(first_pos + 1, 0), end), clear_from = p.window ? (int)max(0ll, (long long)last_pos - (long long)p.window + 1) : 0;
 
-            float acc[D / 16][NT][4], off[NT][2][NG], l[NT][2], m[NT][2], fv[NG];
+            float acc[D / 16][NT][4], off[NT][2][NG], l[NT][2], m[NT][2];
+            float fv[NG], limit[NG];                         // factor of the steps, and the step that it is good for
 #pragma unroll
             for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -302,6 +309,7 @@ __global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 fv[g] = 0.0f;
+                limit[g] = -1.0f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) off[nt][0][g] = off[nt][1][g] = 0.0f;
             }
@@ -310,125 +318,127 @@ __global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) { l[nt][i] = 0.0f; m[nt][i] = -INFINITY; }
 
-            // ---- this warp's cells: c0 + warp, + 4, ...
-            const int count = (c1 - c0 - warp + kDecodeWarps - 1) / kDecodeWarps;
-            unsigned long long page_at = 0;                  // of the cell j0 + lane
-            auto pages_of = [&](int j0) {
-                const int c = rq.first + c0 + warp + kDecodeWarps * (j0 + lane);
-                page_at = 0;
-                if (j0 + lane < count && c * kCellTokens < rq.length) {
+            // ---- this warp's steps: cells c0 + 2 (warp + 4 j), + 1
+            const int count = ((c1 - c0 + 1) / 2 - warp + kDecodeWarps - 1) / kDecodeWarps;
+            uint32_t cell_at = kNoCell;                      // place in the cache of the cell 2 j0 + lane of this warp's steps
+            auto places_of = [&](int j0) {
+                const int c = rq.first + c0 + 2 * (warp + kDecodeWarps * (j0 + (lane >> 1))) + (lane & 1);
+                cell_at = kNoCell;
+                if (c < rq.first + c1 && c * kCellTokens < rq.length) {
                     const uint32_t column = (uint32_t)c / p.page_cells;
                     const int page = p.table[(long long)b * p.table_stride + column];
-                    if (page >= 0 && (uint32_t)page < p.pages)
-                        page_at = (unsigned long long)(p.cache + ((size_t)page * p.kv_heads + head) * p.page_bytes + (size_t)((uint32_t)c % p.page_cells) * CELL);
-                    else
-                        raise_error(p.err, kErrKv4Page);
+                    if (page >= 0 && (uint32_t)page < p.pages) cell_at = ((uint32_t)page * p.kv_heads + head) * p.page_cells + (uint32_t)c % p.page_cells;
+                    else raise_error(p.err, kErrKv4Page);
                 }
             };
+            uint32_t fill = ring_s + lane * 16u;
             auto issue = [&](int j) {
                 if (j < count) {
-                    if ((j & 31) == 0) pages_of(j);
-                    const unsigned long long at = __shfl_sync(0xffffffffu, page_at, j & 31);
-                    const uint32_t dst = ring_s + (uint32_t)(j % STAGES) * CELL;
-                    const uint8_t* src = at ? reinterpret_cast<const uint8_t*>(at) : p.cache;
-                    const uint32_t bytes = at ? 16u : 0u;
+                    if ((j & 15) == 0) places_of(j);
 #pragma unroll
-                    for (uint32_t i = 0; i < (CELL / 16 + 31) / 32; ++i) {
-                        const uint32_t o = (i * 32 + lane) * 16u;
-                        if (CELL % 512 == 0 || o < CELL) cp_async16(dst + o, src + (at ? o : 0), bytes);
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t at = __shfl_sync(0xffffffffu, cell_at, 2 * (j & 15) + u);
+                        const uint32_t bytes = at == kNoCell ? 0u : 16u;       // zeros, from a source that is not read
+                        const uint8_t* src = p.cache + (size_t)(at == kNoCell ? 0u : at) * CELL + lane * 16u;
+#pragma unroll
+                        for (uint32_t i = 0; i < (CELL / 16 + 31) / 32; ++i)
+                            if (CELL % 512 == 0 || i * 512u + lane * 16u < CELL) cp_async16(fill + u * CELL + i * 512u, src + i * 512u, bytes);
                     }
+                    fill = fill == ring_s + lane * 16u + (kStages - 1) * 2u * CELL ? ring_s + lane * 16u : fill + 2u * CELL;
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
+            // One step.  CLEAR: every row of the tile sees all 32 tokens.
+            auto step = [&](const uint8_t* st, int tok0, auto clear_tag) {
+                constexpr bool CLEAR = decltype(clear_tag)::value;
+                constexpr int PER = NW < 4 ? NW : 4;          // words of a lane in a block
+                constexpr int VB = D < 128 ? 1 : D / 128, VP = NW / VB;      // blocks of values, words of a lane and plane in each
+                // ---- scores: rows = tokens gid, gid + 8 of cell u; columns = queries 2 tig, 2 tig + 1
+                float s[2][NT][4];
+                uint32_t vr[2][2][NG];                        // steps and offsets of the values
 #pragma unroll
-            for (int j = 0; j < STAGES - 1; ++j) issue(j);
-            for (int j = 0; j < count; ++j) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-                __syncwarp();
-                issue(j + STAGES - 1);                       // into the stage that the last step read
-                const uint8_t* st = ring + (size_t)(j % STAGES) * CELL;
-                const int tok0 = (rq.first + c0 + warp + kDecodeWarps * j) * kCellTokens;
-                const bool clear = tok0 >= clear_from && tok0 + kCellTokens <= clear_to;
-
-                // steps and offsets of the tokens gid, gid + 8
-                float ks[NG][2], ko[NG][2], vs[NG][2], vo[NG][2];
+                for (int u = 0; u < 2; ++u) {
+                    const uint8_t* cell = st + u * CELL;
+                    uint32_t kr[2][NG];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const bool inside = tok0 + gid + 8 * i < rq.length;      // behind the end lies what the page held before
-                    uint32_t a[NG], c[NG];
-                    load_words(a, st + kv4_key_step(D, GS, gid + 8 * i, 0));
-                    load_words(c, st + kv4_value_step(D, GS, gid + 8 * i, 0));
+                    for (int i = 0; i < 2; ++i) {
+                        load_words(kr[i], cell + kv4_key_step(D, GS, gid + 8 * i, 0));
+                        load_words(vr[u][i], cell + kv4_value_step(D, GS, gid + 8 * i, 0));
+                        if (!CLEAR && tok0 + 16 * u + 8 * i + gid >= rq.length) {      // behind the end lies what the page held before
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) kr[i][g] = vr[u][i][g] = 0u;
+                        }
+                    }
+                    uint32_t xa[NW / PER][PER], xb[NW / PER][PER];
+#pragma unroll
+                    for (int bl = 0; bl < NW / PER; ++bl) {
+                        load_words(xa[bl], cell + ((bl * 16 + gid) * 4 + tig) * PER * 4);
+                        load_words(xb[bl], cell + ((bl * 16 + gid + 8) * 4 + tig) * PER * 4);
+                    }
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        if (!inside) a[g] = c[g] = 0u;
-                        const float2 fa = unpack2<DT>(a[g]), fc = unpack2<DT>(c[g]);
-                        ks[g][i] = fa.x; ko[g][i] = fmaf(8.0f, fa.x, fa.y);
-                        vs[g][i] = fc.x; vo[g][i] = fmaf(8.0f, fc.x, fc.y);
-                    }
-                }
-                // ---- scores: rows = tokens gid, gid + 8; columns = queries 2 tig, 2 tig + 1
-                float s[NT][4];
+                        float raw[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][i] = 0.0f;
-                constexpr int PER = NW < 4 ? NW : 4;          // words of a lane in a block
-                uint32_t xa[NW / PER][PER], xb[NW / PER][PER];
+                            for (int i = 0; i < 4; ++i) raw[nt][i] = 0.0f;
 #pragma unroll
-                for (int bl = 0; bl < NW / PER; ++bl) {
-                    load_words(xa[bl], st + ((bl * 16 + gid) * 4 + tig) * PER * 4);
-                    load_words(xb[bl], st + ((bl * 16 + gid + 8) * 4 + tig) * PER * 4);
-                }
+                        for (int w = g * GS / 32; w < (g + 1) * GS / 32; ++w) {
+                            uint32_t ca[4], cb[4];
+                            code_pairs(xa[w / PER][w % PER], ca);
+                            code_pairs(xb[w / PER][w % PER], cb);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    float raw[NT][4];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) raw[nt][i] = 0.0f;
-#pragma unroll
-                    for (int w = g * GS / 32; w < (g + 1) * GS / 32; ++w) {
-                        uint32_t ca[4], cb[4];
-                        code_pairs(xa[w / PER][w % PER], ca);
-                        code_pairs(xb[w / PER][w % PER], cb);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma_16816<FP16>(raw[nt], ca[0], cb[0], ca[1], cb[1], qf[nt][w][0], qf[nt][w][1]);
-                            mma_16816<FP16>(raw[nt], ca[2], cb[2], ca[3], cb[3], qf[nt][w][2], qf[nt][w][3]);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma_16816<FP16>(raw[nt], ca[0], cb[0], ca[1], cb[1], qf[nt][w][0], qf[nt][w][1]);
+                                mma_16816<FP16>(raw[nt], ca[2], cb[2], ca[3], cb[3], qf[nt][w][2], qf[nt][w][3]);
+                            }
                         }
-                    }
+                        float ks[2], ko[2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s[nt][i] = fmaf(raw[nt][i], ks[g][i >> 1], s[nt][i]);
-                            s[nt][i] = fmaf(ko[g][i >> 1], qs[nt][i & 1][g], s[nt][i]);
+                        for (int i = 0; i < 2; ++i) {
+                            const float2 f = unpack2<DT>(kr[i][g]);
+                            ks[i] = f.x;
+                            ko[i] = fmaf(8.0f, f.x, f.y);
                         }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float middle = ko[i >> 1] * qs[nt][i & 1][g];
+                                s[u][nt][i] = fmaf(raw[nt][i], ks[i >> 1], g == 0 ? middle : s[u][nt][i] + middle);
+                            }
+                    }
                 }
                 bool follow = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[nt][i] *= sf[nt][i & 1];
-                        if (!clear) {
-                            const int tok = tok0 + gid + 8 * (i >> 1);
-                            if (tok < from[nt][i & 1] || tok >= to[nt][i & 1]) s[nt][i] = -INFINITY;
-                        }
-                    }
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) follow |= fmaxf(s[nt][i], s[nt][2 + i]) > m[nt][i] + kGrow;
+                        for (int i = 0; i < 4; ++i) {
+                            s[u][nt][i] *= sf[nt][i & 1];
+                            if (!CLEAR) {
+                                const int tok = tok0 + 16 * u + gid + 8 * (i >> 1);
+                                if (tok < from[nt][i & 1] || tok >= to[nt][i & 1]) s[u][nt][i] = -INFINITY;
+                            }
+                        }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        follow |= fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i])) > m[nt][i] + kGrow;
                 }
 #pragma unroll
-                for (int g = 0; g < NG; ++g) follow |= fmaxf(vs[g][0], vs[g][1]) * fv[g] > 2048.0f || fv[g] == 0.0f;
+                for (int g = 0; g < NG; ++g) {
+                    const float top = fmaxf(fmaxf(unpack2<DT>(vr[0][0][g]).x, unpack2<DT>(vr[0][1][g]).x), fmaxf(unpack2<DT>(vr[1][0][g]).x, unpack2<DT>(vr[1][1][g]).x));
+                    follow |= top > limit[g];
+                }
                 if (__any_sync(0xffffffffu, follow)) {
-                    // maxima over the cell, sums brought to them; rare once a few cells are done
+                    // maxima over the step, sums brought to them; rare once a few cells are done
                     float down[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float top = fmaxf(s[nt][i], s[nt][2 + i]);
+                            float top = fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i]));
 #pragma unroll
                             for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             top = fmaxf(top, m[nt][i]);
@@ -438,13 +448,16 @@ __global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
                         }
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs[g][0], vs[g][1])));
-                        int e = (int)(bits >> 23) - 127;               // the largest step is below 2^(e+1)
-                        e = max(e, -100);
-                        const float want = pow2(10 - min(e, 100));
+                        const float top = fmaxf(fmaxf(unpack2<DT>(vr[0][0][g]).x, unpack2<DT>(vr[0][1][g]).x), fmaxf(unpack2<DT>(vr[1][0][g]).x, unpack2<DT>(vr[1][1][g]).x));
+                        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(top, 0.0f)));
+                        const int e = min(max((int)(bits >> 23) - 127, -100), 100);   // the largest step is below 2^(e+1)
+                        const float want = pow2(10 - e);
                         float by = 1.0f;
-                        if (fv[g] == 0.0f) fv[g] = want;
-                        else if (want < fv[g]) { by = want / fv[g]; fv[g] = want; }
+                        if (limit[g] < 0.0f || want < fv[g]) {
+                            by = limit[g] < 0.0f ? 0.0f : want / fv[g];               // the sums are still 0 at first
+                            fv[g] = want;
+                            limit[g] = pow2(e + 1);
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             const float d0 = by * down[nt][0], d1 = by * down[nt][1];
@@ -457,56 +470,73 @@ __global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
                         }
                     }
                 }
-                float w[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int u = 0; u < 2; ++u) {
+                    const uint8_t* cell = st + u * CELL;
+                    float w[NT][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        // a row that has seen nothing yet has the maximum -inf: its weights are 0
-                        w[nt][i] = (!clear && s[nt][i] == -INFINITY) ? 0.0f : ex2(s[nt][i] - m[nt][i & 1]);
-                        l[nt][i & 1] += w[nt][i];
-                    }
-                // the lane's value codes: both planes (tokens 0..7, 8..15)
-                constexpr int VB = D < 128 ? 1 : D / 128, VP = NW / VB;      // blocks, words of a lane and plane in each
-                uint32_t xv[VB][2][VP];
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int bl = 0; bl < VB; ++bl)
+                        for (int i = 0; i < 4; ++i) {
+                            // a row that has seen nothing yet has the maximum -inf: its weights are 0
+                            w[nt][i] = (!CLEAR && s[u][nt][i] == -INFINITY) ? 0.0f : ex2(s[u][nt][i] - m[nt][i & 1]);
+                            l[nt][i & 1] += w[nt][i];
+                        }
+                    // ---- outputs: rows = elements, depth = tokens, columns = queries; planes of tokens 0..7 and 8..15
+                    uint32_t xv[VB][2][VP];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) load_words(xv[bl][c], st + 8 * D + ((bl * 2 + c) * 32 + lane) * (VP * 4));
-                // ---- outputs: rows = elements, depth = tokens, columns = queries
+                    for (int bl = 0; bl < VB; ++bl)
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    uint32_t b0[NT], b1[NT];
-                    const float f0 = vs[g][0] * fv[g], f1 = vs[g][1] * fv[g];
+                        for (int c = 0; c < 2; ++c) load_words(xv[bl][c], cell + 8 * D + ((bl * 2 + c) * 32 + lane) * (VP * 4));
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        b0[nt] = movmatrix(half2_bits(w[nt][0] * f0, w[nt][1] * f0));
-                        b1[nt] = movmatrix(half2_bits(w[nt][2] * f1, w[nt][3] * f1));
+                    for (int g = 0; g < NG; ++g) {
+                        uint32_t b0[NT], b1[NT];
+                        const float2 v0 = unpack2<DT>(vr[u][0][g]), v1 = unpack2<DT>(vr[u][1][g]);
+                        const float f0 = v0.x * fv[g], f1 = v1.x * fv[g], o0 = fmaf(8.0f, v0.x, v0.y), o1 = fmaf(8.0f, v1.x, v1.y);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            if (clear) {
-                                off[nt][i][g] = fmaf(w[nt][i], vo[g][0], fmaf(w[nt][2 + i], vo[g][1], off[nt][i][g]));
-                            } else {                         // a token that this row does not see may hold no number
-                                off[nt][i][g] += w[nt][i] == 0.0f ? 0.0f : w[nt][i] * vo[g][0];
-                                off[nt][i][g] += w[nt][2 + i] == 0.0f ? 0.0f : w[nt][2 + i] * vo[g][1];
+                        for (int nt = 0; nt < NT; ++nt) {
+                            b0[nt] = movmatrix(half2_bits(w[nt][0] * f0, w[nt][1] * f0));
+                            b1[nt] = movmatrix(half2_bits(w[nt][2] * f1, w[nt][3] * f1));
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                if (CLEAR) {
+                                    off[nt][i][g] = fmaf(w[nt][i], o0, fmaf(w[nt][2 + i], o1, off[nt][i][g]));
+                                } else {                     // a token that this row does not see may hold no number
+                                    off[nt][i][g] += w[nt][i] == 0.0f ? 0.0f : w[nt][i] * o0;
+                                    off[nt][i][g] += w[nt][2 + i] == 0.0f ? 0.0f : w[nt][2 + i] * o1;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int i = g * GS / 32; i < (g + 1) * GS / 32; ++i) {      // elements 32 i .. + 31, four of them in the lane's word
+                            uint32_t c0v[4], c1v[4];
+                            code_pairs(xv[i / VP][0][i % VP], c0v);
+                            code_pairs(xv[i / VP][1][i % VP], c1v);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma_16816<FP16>(acc[2 * i][nt], c0v[0], c0v[1], c1v[0], c1v[1], b0[nt], b1[nt]);
+                                mma_16816<FP16>(acc[2 * i + 1][nt], c0v[2], c0v[3], c1v[2], c1v[3], b0[nt], b1[nt]);
                             }
                         }
                     }
-#pragma unroll
-                    for (int i = g * GS / 32; i < (g + 1) * GS / 32; ++i) {      // elements 32 i .. + 31, four of them in the lane's word
-                        uint32_t c0v[4], c1v[4];
-                        code_pairs(xv[i / VP][0][i % VP], c0v);
-                        code_pairs(xv[i / VP][1][i % VP], c1v);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma_16816<FP16>(acc[2 * i][nt], c0v[0], c0v[1], c1v[0], c1v[1], b0[nt], b1[nt]);
-                            mma_16816<FP16>(acc[2 * i + 1][nt], c0v[2], c0v[3], c1v[2], c1v[3], b0[nt], b1[nt]);
-                        }
-                    }
                 }
+            };
+#pragma unroll
+            for (int j = 0; j < kStages - 1; ++j) issue(j);
+            const uint8_t* st = ring;
+            int tok0 = (rq.first + c0 + 2 * warp) * kCellTokens;
+            for (int j = 0; j < count; ++j) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+                __syncwarp();
+                issue(j + kStages - 1);                      // into the stage that the last step read
+                // behind the end of the segment's cells lies another block's work: `to` hides it
+                if (tok0 >= clear_from && tok0 + 2 * kCellTokens <= clear_to) step(st, tok0, std::true_type{});
+                else step(st, tok0, std::false_type{});
+                st = st == ring + (kStages - 1) * 2 * CELL ? ring : st + 2 * CELL;
+                tok0 += kDecodeWarps * 2 * kCellTokens;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            __syncwarp();
+            __syncthreads();                                 // every warp is through with its ring
 
             // ---- the warps' sums into shared memory
 #pragma unroll
@@ -683,10 +713,8 @@ template <int D, int GS, int NT, int DT> int decode_blocks_per_sm() {
 
 template <int D, int GS, int NT, int DT> cudaError_t run_decode(const Kv4Attn& p, uint32_t blocks, cudaStream_t s) {
     if (!decode_blocks_per_sm<D, GS, NT, DT>()) return cudaErrorInvalidConfiguration;
-    kv4_decode_kernel<D, GS, NT, DT><<<blocks, kDecodeThreads, decode_smem<D, GS, NT>(), s>>>(p);
-    if (cudaError_t e = cudaGetLastError()) return e;
-    kv4_join_kernel<D, NT, DT><<<dim3(blocks, 8 * NT), 128, 0, s>>>(p, blocks);
-    return cudaGetLastError();
+    if (cudaError_t e = launch_early(kv4_decode_kernel<D, GS, NT, DT>, dim3(blocks), dim3(kDecodeThreads), decode_smem<D, GS, NT>(), s, p)) return e;
+    return launch_early(kv4_join_kernel<D, NT, DT>, dim3(blocks, 8 * NT), dim3(128), 0, s, p, blocks);
 }
 
 // f<GS, NT, DT>() of a head size
