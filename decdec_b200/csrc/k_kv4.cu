@@ -14,64 +14,86 @@ constexpr uint32_t kMaxRotaryPairs = 512;
 // (a, b) -> ((a cos - b sin) f, (b cos + a sin) f), angle = position * frequency.  Bound by memory: 16-bit rows are read and
 // written once, V pairs (2 V elements, 16 bytes a half) per thread and step.  The angle is taken in 64 bits, where a position of a
 // million still has 2^-33 of a turn, reduced to one turn there, and its sine and cosine in 32 bits: once per token and pair, in
-// shared memory for all heads.
+// shared memory for all heads.  A block takes `span` tokens, so that its threads have an angle each, and reads its first rows before
+// it computes them.
 template <int DT, bool HALF, int V>
 __global__ void __launch_bounds__(256) rotary_kernel(Rows q, uint32_t q_heads, Rows k, uint32_t k_heads, Rows qo, Rows ko, const void* positions,
                                                      int wide, const double* __restrict__ frequencies, uint32_t tokens, uint32_t head_dim,
-                                                     uint32_t rotary_dim, float factor) {
+                                                     uint32_t rotary_dim, uint32_t span, float factor) {
     using T = typename Tr<DT>::T;
-    __shared__ float2 turn[kMaxRotaryPairs];
+    extern __shared__ float2 turn[];                          // [span][rotary_dim / 2]
     struct alignas(sizeof(T) * V) Vec { T v[V]; };
     pdl_trigger();
     pdl_wait();
     const uint32_t pairs = rotary_dim / 2u;
-    const uint32_t t = blockIdx.x;
-    const long long pos = wide ? reinterpret_cast<const long long*>(positions)[t] : (long long)reinterpret_cast<const int*>(positions)[t];
-    for (uint32_t i = threadIdx.x; i < pairs; i += blockDim.x) {
-        const double turns = (double)pos * frequencies[i] * 0.15915494309189533576888;     // 1 / 2 pi
+    const uint32_t t0 = blockIdx.x * span, n = min(span, tokens - t0);
+    // steps of a head: pairs / V that turn, then (head_dim - rotary_dim) / 2V that are copied
+    const uint32_t turning = pairs / V, steps = head_dim / (2u * V), per_token = (q_heads + k_heads) * steps, total = n * per_token;
+    struct At { const T* src; T* dst; uint32_t at0, at1, angle; bool turns; };
+    auto place = [&](uint32_t j) {
+        const uint32_t t = span == 1u ? 0u : j / per_token;
+        const uint32_t in = j - t * per_token;
+        uint32_t h = in / steps;
+        const uint32_t e = in - h * steps;
+        const bool is_k = h >= q_heads;
+        if (is_k) h -= q_heads;
+        At a;
+        a.src = reinterpret_cast<const T*>(is_k ? k.p : q.p) + (long long)(t0 + t) * (is_k ? k.token : q.token) + (long long)h * (is_k ? k.head : q.head);
+        a.dst = reinterpret_cast<T*>(const_cast<void*>(is_k ? ko.p : qo.p)) + (long long)(t0 + t) * (is_k ? ko.token : qo.token) +
+                (long long)h * (is_k ? ko.head : qo.head);
+        a.turns = e < turning;
+        // half layout: the two halves of a pair are rotary_dim / 2 apart; else, and where elements are only copied, neighbours
+        a.at0 = (HALF && a.turns) ? e * V : e * 2u * V;
+        a.at1 = (HALF && a.turns) ? a.at0 + pairs : a.at0 + V;
+        a.angle = t * pairs + e * V;
+        return a;
+    };
+    uint32_t j = blockIdx.y * blockDim.x + threadIdx.x;
+    At at = {};
+    Vec x, y;
+    if (j < total) {
+        at = place(j);
+        x = *reinterpret_cast<const Vec*>(at.src + at.at0);
+        y = *reinterpret_cast<const Vec*>(at.src + at.at1);
+    }
+    for (uint32_t i = threadIdx.x; i < n * pairs; i += blockDim.x) {
+        const uint32_t t = t0 + i / pairs;
+        const long long pos = wide ? reinterpret_cast<const long long*>(positions)[t] : (long long)reinterpret_cast<const int*>(positions)[t];
+        const double turns = (double)pos * frequencies[i % pairs] * 0.15915494309189533576888;     // 1 / 2 pi
         float s, c;
         sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
         turn[i] = make_float2(c, s);
     }
     __syncthreads();
-    // steps of a head: pairs / V that turn, then (head_dim - rotary_dim) / 2V that are copied
-    const uint32_t turning = pairs / V, steps = head_dim / (2u * V);
-    const uint32_t total = (q_heads + k_heads) * steps;
-    for (uint32_t j = blockIdx.y * blockDim.x + threadIdx.x; j < total; j += blockDim.x * gridDim.y) {
-        uint32_t h = j / steps;
-        const uint32_t e = j % steps;
-        const bool is_k = h >= q_heads;
-        if (is_k) h -= q_heads;
-        const T* src = reinterpret_cast<const T*>(is_k ? k.p : q.p) + (long long)t * (is_k ? k.token : q.token) + (long long)h * (is_k ? k.head : q.head);
-        T* dst = reinterpret_cast<T*>(const_cast<void*>(is_k ? ko.p : qo.p)) + (long long)t * (is_k ? ko.token : qo.token) +
-                 (long long)h * (is_k ? ko.head : qo.head);
-        const bool turns = e < turning;
-        // half layout: the two halves of a pair are rotary_dim / 2 apart; else, and where elements are only copied, neighbours
-        const uint32_t at0 = (HALF && turns) ? e * V : e * 2u * V;
-        const uint32_t at1 = (HALF && turns) ? at0 + pairs : at0 + V;
-        Vec x = *reinterpret_cast<const Vec*>(src + at0), y = *reinterpret_cast<const Vec*>(src + at1);
-        if (turns) {
+    while (j < total) {
+        if (at.turns) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 T& xa = HALF ? x.v[i] : (2 * i < V ? x.v[(2 * i) % V] : y.v[(2 * i) % V]);
                 T& xb = HALF ? y.v[i] : (V == 1 ? y.v[0] : (2 * i < V ? x.v[(2 * i + 1) % V] : y.v[(2 * i + 1) % V]));
-                const float2 cs = turn[e * V + i];
+                const float2 cs = turn[at.angle + i];
                 const float a = Tr<DT>::to_f(xa), b = Tr<DT>::to_f(xb);
                 xa = Tr<DT>::from_f((a * cs.x - b * cs.y) * factor);
                 xb = Tr<DT>::from_f((b * cs.x + a * cs.y) * factor);
             }
         }
-        *reinterpret_cast<Vec*>(dst + at0) = x;
-        *reinterpret_cast<Vec*>(dst + at1) = y;
+        *reinterpret_cast<Vec*>(at.dst + at.at0) = x;
+        *reinterpret_cast<Vec*>(at.dst + at.at1) = y;
+        j += blockDim.x * gridDim.y;
+        if (j < total) {
+            at = place(j);
+            x = *reinterpret_cast<const Vec*>(at.src + at.at0);
+            y = *reinterpret_cast<const Vec*>(at.src + at.at1);
+        }
     }
 }
 
 template <int DT, bool HALF>
-cudaError_t rotary_any(int vec, dim3 grid, cudaStream_t s, const Rows& q, uint32_t qh, const Rows& k, uint32_t kh, const Rows& qo, const Rows& ko,
+cudaError_t rotary_any(int vec, dim3 grid, uint32_t span, cudaStream_t s, const Rows& q, uint32_t qh, const Rows& k, uint32_t kh, const Rows& qo, const Rows& ko,
                        const void* positions, int wide, const double* f, uint32_t tokens, uint32_t d, uint32_t r, float factor) {
     constexpr int W = DT == FP32 ? 4 : 8;
-    return launch_early(vec ? rotary_kernel<DT, HALF, W> : rotary_kernel<DT, HALF, 1>, grid, dim3(256), 0, s, q, qh, k, kh, qo, ko, positions, wide, f, tokens, d, r,
-                        factor);
+    return launch_early(vec ? rotary_kernel<DT, HALF, W> : rotary_kernel<DT, HALF, 1>, grid, dim3(256), (size_t)span * r / 2u * sizeof(float2), s, q, qh, k, kh, qo, ko,
+                        positions, wide, f, tokens, d, r, span, factor);
 }
 
 // ---- plan of a step --------------------------------------------------------------------------------------
@@ -186,171 +208,245 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Plan p) {
 }
 
 // ---- rows into the cache -----------------------------------------------------------------------------------
-// min / max over groups of L neighbouring lanes
-template <int L>
-__device__ __forceinline__ void group_range(float& lo, float& hi) {
-#pragma unroll
-    for (int o = 1; o < L; o *= 2) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-}
-
 template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     typename Tr<DT>::T v[2] = {Tr<DT>::from_f(a), Tr<DT>::from_f(b)};
     return *reinterpret_cast<const uint32_t*>(v);
 }
+template <int DT> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+    if constexpr (DT == FP16) {
+        const __half2 r = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        const __nv_bfloat162 r = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+// whether one of the two 16-bit values is infinite or NaN
+template <int DT> __device__ __forceinline__ uint32_t no_number(uint32_t v) {
+    constexpr uint32_t E = DT == FP16 ? 0x7c007c00u : 0x7f807f80u, U = DT == FP16 ? 0x04000400u : 0x00800080u;
+    return ((v & E) + U) & 0x80008000u;
+}
 
-// code of x in steps from lo, the nearest, ties to even, exactly as over the reals: a first guess by a product, then the two
-// comparisons with its borders in exact arithmetic (difference of halves with its rounding error; border * step has 16 bits).
-// Everything is halved so that the range of a bf16 group does not overflow.
-__device__ __forceinline__ uint32_t code_of(float xh, float loh, float steph, float inv) {
+// code of x in steps from lo, the nearest, ties to even, exactly as over the reals: the two comparisons of the guess n with its borders in
+// exact arithmetic (difference with its rounding error; border * step has 16 bits).  All arguments halved, so that the range of a bf16
+// group does not overflow.
+__device__ __forceinline__ float exact_code(float xh, float loh, float steph, float n) {
     const float d = xh - loh;
     const float back = d + loh;                                  // two-difference: xh - loh = d + e
     const float e = (xh - back) + ((back - d) - loh);
-    const float guess = inv != 0.0f ? d * inv : d / steph;
-    float n = fminf(fmaxf(rintf(guess), 0.0f), 15.0f);
+    n = fminf(fmaxf(n, 0.0f), 15.0f);
     const bool odd = ((int)n & 1) != 0;
     const float above = fmaf(-(n + 0.5f), steph, d) + e, below = fmaf(-(n - 0.5f), steph, d) + e;
     if (above > 0.0f || (above == 0.0f && odd)) n += 1.0f;
     else if (below < 0.0f || (below == 0.0f && odd)) n -= 1.0f;
-    return (uint32_t)fminf(fmaxf(n, 0.0f), 15.0f);
+    return fminf(fmaxf(n, 0.0f), 15.0f);
 }
 
-// Bound by memory (2 bytes an element in, half a byte out), with about 25 instructions an element beside it.  A lane takes the four
-// elements of a 16-bit word of keys and of values, so 128 elements of a head are one coalesced 256-byte read of each and the group
-// extremes are a few shuffles.
+// (hi - lo) / 15 rounded to the type, of halves.  The quotient by a constant is corrected by its remainder, which rounds as a division does
+// (Markstein's theorem) where nothing underflows.
+template <int DT> __device__ __forceinline__ float step_of(float lo, float hi) {
+    const float range = 0.5f * hi - 0.5f * lo;
+    float q = range * (1.0f / 7.5f);
+    q = fmaf(fmaf(-q, 7.5f, range), 1.0f / 7.5f, q);
+    if (range < 1e-30f) q = range / 7.5f;
+    return Tr<DT>::to_f(Tr<DT>::from_f(q));
+}
+
+// four codes of 16-bit values a, b in a 16-bit word
+template <int DT> __device__ __forceinline__ uint32_t code_word(uint32_t a, uint32_t b, float lo, float step) {
+    if (!(step > 0.0f)) return 0u;
+    const float2 fa = unpack2<DT>(a), fb = unpack2<DT>(b);
+    const float h[4] = {0.5f * fa.x, 0.5f * fa.y, 0.5f * fb.x, 0.5f * fb.y};
+    const float loh = 0.5f * lo, steph = 0.5f * step;
+    const bool small = steph < 1e-30f;                           // its reciprocal may overflow
+    float inv;                                                   // a guess: what it is off by stays far below `near`
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(steph));
+    if (small) inv = 0.0f;
+    const float near = steph * 0.4999f;
+    uint32_t word = 0;
+    bool border = small;
+    float n[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float d = h[j] - loh;
+        const float up = fmaf(d, inv, 12582912.0f);              // 1.5 * 2^23: the sum's last bits are the rounded quotient
+        n[j] = up - 12582912.0f;
+        border |= fabsf(fmaf(-n[j], steph, d)) > near || n[j] > 15.0f;       // next to a border; beyond the last code (subnormal steps)
+        word |= (__float_as_uint(up) & 15u) << (4 * j);
+    }
+    if (border) {                                                // of the four, about one in 2^10 random ones; more in short types
+        word = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) word |= (uint32_t)exact_code(h[j], loh, steph, small ? rintf((h[j] - loh) / steph) : n[j]) << (4 * j);
+    }
+    return word;
+}
+
+// where a slot lies: the first head's cell and the token's place in it
+struct Place {
+    uint8_t* cell;
+    uint32_t r;
+    bool inside;
+};
+__device__ __forceinline__ Place place_of(const Kv4Cache& c, const void* slots, int wide, uint32_t t, uint32_t cell_bytes, bool report, unsigned* err) {
+    const long long slot = wide ? reinterpret_cast<const long long*>(slots)[t] : (long long)reinterpret_cast<const int*>(slots)[t];
+    const uint32_t page_tokens = c.page_cells * kCellTokens;
+    Place p;
+    p.inside = slot >= 0 && slot < (long long)c.pages * page_tokens;
+    if (slot >= 0 && !p.inside && report) raise_error(err, kErrKv4Page);
+    const uint32_t page = p.inside ? quotient((size_t)slot, page_tokens) : 0u;
+    const uint32_t in_page = p.inside ? (uint32_t)((size_t)slot - (size_t)page * page_tokens) : 0u;
+    p.cell = c.data + (size_t)page * c.kv_heads * c.page_bytes + (size_t)(in_page / kCellTokens) * cell_bytes;
+    p.r = in_page % kCellTokens;
+    return p;
+}
+
+// A warp takes a token and `rounds` warps' widths of its heads; a lane the four elements of a 16-bit word of keys and of values, so 128
+// elements of a head are one coalesced 256-byte read of each, and the group extremes are a few shuffles of (least, -largest) pairs.  Bound
+// by the instructions, about 15 an element: the slot is looked up once for all heads, ties are settled apart.
 template <int DT, int D, int GS, bool VEC>
-__global__ void __launch_bounds__(256) append_kernel(Rows k, Rows v, const void* slots, int wide, Kv4Cache c, uint32_t tokens, unsigned* err) {
+__global__ void __launch_bounds__(256) append_kernel(Rows k, Rows v, const void* slots, int wide, Kv4Cache c, uint32_t tokens, uint32_t chunks, uint32_t rounds,
+                                                     unsigned* err) {
     using T = typename Tr<DT>::T;
     constexpr uint32_t BL = D < 128 ? D : 128;          // elements of a unit
     constexpr uint32_t LANES = BL / 4;                   // lanes of a unit
     constexpr uint32_t UNITS = D / BL;                   // units of a head
+    constexpr uint32_t PER_WARP = 32 / LANES;
     constexpr int GL = GS / 4;                           // lanes of a group
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t units = (uint64_t)tokens * c.kv_heads * UNITS;
-    constexpr uint32_t PER_WARP = 32 / LANES;
-    const uint64_t warps = (uint64_t)gridDim.x * (blockDim.x / 32u);
-    const uint64_t rounds = (units + PER_WARP - 1) / PER_WARP;
-    for (uint64_t i = (uint64_t)blockIdx.x * (blockDim.x / 32u) + (threadIdx.x >> 5); i < rounds; i += warps) {
-        const uint64_t unit = i * PER_WARP + lane / LANES;
-        const bool live = unit < units;
-        const uint32_t th = live ? (uint32_t)(unit / UNITS) : 0u;
-        const uint32_t t = th / c.kv_heads, h = th % c.kv_heads;
-        const uint32_t u = (UNITS > 1 ? (uint32_t)(unit % UNITS) * (BL / 4) : 0u) + lane % LANES;
-        const long long slot = wide ? reinterpret_cast<const long long*>(slots)[t] : (long long)reinterpret_cast<const int*>(slots)[t];
-        const uint32_t page_tokens = c.page_cells * kCellTokens;
-        const bool inside = slot >= 0 && slot < (long long)c.pages * page_tokens;
-        if (live && slot >= 0 && !inside && lane % LANES == 0u) raise_error(err, kErrKv4Page);
-        const long long page = inside ? slot / page_tokens : 0;
-        const uint32_t in_page = inside ? (uint32_t)(slot % page_tokens) : 0u;
-        uint8_t* cell = c.data + ((size_t)page * c.kv_heads + h) * c.page_bytes + (size_t)(in_page / kCellTokens) * kv4_cell_bytes(D, GS);
-        const uint32_t r = in_page % kCellTokens;
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const Rows& x = side ? v : k;
-            const T* src = reinterpret_cast<const T*>(x.p) + (long long)t * x.token + (long long)h * x.head + 4u * u;
-            float f[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t lane = threadIdx.x & 31u, all = c.kv_heads * UNITS;
+    const uint64_t items = (uint64_t)tokens * chunks;
+    for (uint64_t i = (uint64_t)blockIdx.x * (blockDim.x / 32u) + (threadIdx.x >> 5); i < items; i += (uint64_t)gridDim.x * (blockDim.x / 32u)) {
+        const uint32_t t = quotient(i, chunks), chunk = (uint32_t)(i - (uint64_t)t * chunks);
+        const Place at = place_of(c, slots, wide, t, kv4_cell_bytes(D, GS), lane == 0u && chunk == 0u, err);
+        if (!at.inside) continue;
+        const uint32_t first = chunk * rounds * PER_WARP + lane / LANES;
+#pragma unroll 2
+        for (uint32_t round = 0; round < rounds; ++round) {
+            const uint32_t unit = first + round * PER_WARP;
+            const bool live = unit < all;
+            const uint32_t h = live ? unit / UNITS : 0u, u = unit % UNITS * (BL / 4) + lane % LANES;
+            uint32_t raw[2][2] = {{0, 0}, {0, 0}};
             if (live) {
-                if constexpr (VEC) {
-                    const uint2 raw = *reinterpret_cast<const uint2*>(src);
-                    const float2 a = unpack2<DT>(raw.x), b = unpack2<DT>(raw.y);
-                    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
-                } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) f[j] = Tr<DT>::to_f(src[j]);
+                for (int side = 0; side < 2; ++side) {
+                    const Rows& x = side ? v : k;
+                    const T* src = reinterpret_cast<const T*>(x.p) + (long long)t * x.token + (long long)h * x.head + 4u * u;
+                    if constexpr (VEC) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(src);
+                        raw[side][0] = w.x; raw[side][1] = w.y;
+                    } else {
+                        const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
+                        raw[side][0] = (uint32_t)e[0] | (uint32_t)e[1] << 16;
+                        raw[side][1] = (uint32_t)e[2] | (uint32_t)e[3] << 16;
+                    }
                 }
             }
-            // an element that is no number makes the range of its group infinite: the group reads back as NaN
-            float lo = INFINITY, hi = -INFINITY;
+            uint8_t* cell = at.cell + (size_t)h * c.page_bytes;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool number = fabsf(f[j]) < INFINITY;
-                lo = fminf(lo, number ? f[j] : -INFINITY);
-                hi = fmaxf(hi, number ? f[j] : INFINITY);
-            }
-            group_range<GL>(lo, hi);
-            float step = Tr<DT>::to_f(Tr<DT>::from_f((0.5f * hi - 0.5f * lo) / 7.5f));
-            if (!(hi < INFINITY) || !(lo > -INFINITY)) { lo = __int_as_float(0x7fc00000); step = 0.0f; }
-            const float steph = 0.5f * step, loh = 0.5f * lo;
-            const float inv = steph >= 1e-30f ? 1.0f / steph : 0.0f;
-            uint32_t word = 0;
-            if (step > 0.0f) {
+            for (int side = 0; side < 2; ++side) {
+                const uint32_t a = raw[side][0], b = raw[side][1];
+                // (least, -largest): a minimum over both signs, then over the lanes of the group; an element that is no number makes the
+                // range infinite, and the group reads back as NaN
+                const uint32_t low = min2<DT>(a, b), high = min2<DT>(a ^ 0x80008000u, b ^ 0x80008000u);
+                uint32_t range = min2<DT>(__byte_perm(low, high, 0x5410), __byte_perm(low, high, 0x7632));
+                if (no_number<DT>(a) | no_number<DT>(b)) range = DT == FP16 ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) word |= code_of(0.5f * f[j], loh, steph, inv) << (4 * j);
-            }
-            if (live && inside) {
-                *reinterpret_cast<uint16_t*>(cell + (side ? kv4_value_word(D, r, u) : kv4_key_word(D, r, u))) = (uint16_t)word;
-                if (u % (GS / 4) == 0u)
-                    *reinterpret_cast<uint32_t*>(cell + (side ? kv4_value_step(D, GS, r, u / (GS / 4)) : kv4_key_step(D, GS, r, u / (GS / 4)))) =
-                        pack2<DT>(step, lo);
+                for (int o = 1; o < GL; o *= 2) range = min2<DT>(range, __shfl_xor_sync(0xffffffffu, range, o));
+                const float2 lh = unpack2<DT>(range);
+                float lo = lh.x, step = step_of<DT>(lo, -lh.y);
+                if (lo == -INFINITY) { lo = __int_as_float(0x7fc00000); step = 0.0f; }
+                const uint32_t word = code_word<DT>(a, b, lo, step);
+                if (live) {
+                    *reinterpret_cast<uint16_t*>(cell + (side ? kv4_value_word(D, at.r, u) : kv4_key_word(D, at.r, u))) = (uint16_t)word;
+                    if (u % (GS / 4) == 0u)
+                        *reinterpret_cast<uint32_t*>(cell + (side ? kv4_value_step(D, GS, at.r, u / (GS / 4)) : kv4_key_step(D, GS, at.r, u / (GS / 4)))) =
+                            pack2<DT>(step, lo);
+                }
             }
         }
     }
 }
 
 // ---- rows out of the cache -----------------------------------------------------------------------------------
+// the smaller, NaN if one is
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Bound by memory.  Warps and lanes as in append.
 template <int DT, int D, int GS>
-__global__ void __launch_bounds__(256) gather_kernel(Kv4Cache c, const void* slots, int wide, void* k_out, void* v_out, uint32_t tokens, unsigned* err) {
+__global__ void __launch_bounds__(256) gather_kernel(Kv4Cache c, const void* slots, int wide, void* k_out, void* v_out, uint32_t tokens, uint32_t chunks,
+                                                     uint32_t rounds, unsigned* err) {
     using T = typename Tr<DT>::T;
+    constexpr uint32_t BL = D < 128 ? D : 128, LANES = BL / 4, UNITS = D / BL, PER_WARP = 32 / LANES;
+    const float most = DT == FP16 ? 65504.0f : 3.38953139e38f;
     pdl_trigger();
     pdl_wait();
-    constexpr uint32_t Q = D / 4;
-    const uint64_t total = (uint64_t)tokens * c.kv_heads * Q;
-    const uint32_t page_tokens = c.page_cells * kCellTokens;
-    const float most = DT == FP16 ? 65504.0f : 3.38953139e38f;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-        const uint64_t th = i / Q;
-        const uint32_t u = (uint32_t)(i % Q);
-        const uint32_t t = (uint32_t)(th / c.kv_heads), h = (uint32_t)(th % c.kv_heads);
-        const long long slot = wide ? reinterpret_cast<const long long*>(slots)[t] : (long long)reinterpret_cast<const int*>(slots)[t];
-        const bool inside = slot >= 0 && slot < (long long)c.pages * page_tokens;
-        if (slot >= 0 && !inside && u == 0u) raise_error(err, kErrKv4Page);
-        const long long page = inside ? slot / page_tokens : 0;
-        const uint32_t in_page = inside ? (uint32_t)(slot % page_tokens) : 0u;
-        const uint8_t* cell = c.data + ((size_t)page * c.kv_heads + h) * c.page_bytes + (size_t)(in_page / kCellTokens) * kv4_cell_bytes(D, GS);
-        const uint32_t r = in_page % kCellTokens, g = u / (GS / 4);
-        uint32_t w[2] = {0, 0}, s[2] = {0, 0};
-        if (inside) {
-            w[0] = *reinterpret_cast<const uint16_t*>(cell + kv4_key_word(D, r, u));
-            w[1] = *reinterpret_cast<const uint16_t*>(cell + kv4_value_word(D, r, u));
-            s[0] = *reinterpret_cast<const uint32_t*>(cell + kv4_key_step(D, GS, r, g));
-            s[1] = *reinterpret_cast<const uint32_t*>(cell + kv4_value_step(D, GS, r, g));
-        }
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const float2 st = unpack2<DT>(s[side]);
-            float f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x = fmaf((float)((w[side] >> (4 * j)) & 15u), st.x, st.y);
-                f[j] = x != x ? x : fminf(fmaxf(x, -most), most);      // a step is rounded: the largest code may lie above the type
+    const uint32_t lane = threadIdx.x & 31u, all = c.kv_heads * UNITS;
+    const uint64_t items = (uint64_t)tokens * chunks;
+    for (uint64_t i = (uint64_t)blockIdx.x * (blockDim.x / 32u) + (threadIdx.x >> 5); i < items; i += (uint64_t)gridDim.x * (blockDim.x / 32u)) {
+        const uint32_t t = quotient(i, chunks), chunk = (uint32_t)(i - (uint64_t)t * chunks);
+        const Place at = place_of(c, slots, wide, t, kv4_cell_bytes(D, GS), lane == 0u && chunk == 0u, err);
+        const uint32_t first = chunk * rounds * PER_WARP + lane / LANES;
+#pragma unroll 2
+        for (uint32_t round = 0; round < rounds; ++round) {
+            const uint32_t unit = first + round * PER_WARP;
+            if (unit >= all) break;
+            const uint32_t h = unit / UNITS, u = unit % UNITS * (BL / 4) + lane % LANES, g = u / (GS / 4);
+            const uint8_t* cell = at.cell + (size_t)h * c.page_bytes;
+            uint32_t w[2] = {0, 0}, s[2] = {0, 0};
+            if (at.inside) {
+                w[0] = *reinterpret_cast<const uint16_t*>(cell + kv4_key_word(D, at.r, u));
+                w[1] = *reinterpret_cast<const uint16_t*>(cell + kv4_value_word(D, at.r, u));
+                s[0] = *reinterpret_cast<const uint32_t*>(cell + kv4_key_step(D, GS, at.r, g));
+                s[1] = *reinterpret_cast<const uint32_t*>(cell + kv4_value_step(D, GS, at.r, g));
             }
-            T* dst = reinterpret_cast<T*>(side ? v_out : k_out) + i * 4u;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]));
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                const float2 st = unpack2<DT>(s[side]);
+                float f[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)                              // 2^23 + code, less 2^23; a rounded step may lead beyond the type
+                    f[j] = min_nan(fmaf(__uint_as_float((w[side] >> (4 * j) & 15u) | 0x4b000000u) - 8388608.0f, st.x, st.y), most);
+                T* dst = reinterpret_cast<T*>(side ? v_out : k_out) + ((size_t)t * c.kv_heads + h) * D + 4u * u;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]));
+            }
         }
     }
 }
 
+// how a token's heads are cut: one warp takes them all while there are tokens enough to fill the device, else fewer
+struct Cut {
+    uint32_t chunks, rounds, blocks;
+};
+Cut cut_heads(uint32_t tokens, uint32_t kv_heads, uint32_t d) {
+    const uint32_t widths = (kv_heads * d + 127u) / 128u;                  // warps' widths of a token
+    const uint32_t want = device_sms() * 96u;                              // warps, three times what an SM holds
+    Cut c;
+    c.chunks = tokens >= want ? 1u : (want + tokens - 1u) / tokens;
+    if (c.chunks > widths) c.chunks = widths;
+    c.rounds = (widths + c.chunks - 1u) / c.chunks;
+    c.chunks = (widths + c.rounds - 1u) / c.rounds;
+    const uint64_t blocks = ((uint64_t)tokens * c.chunks + 7u) / 8u, most = (uint64_t)device_sms() * 8u;
+    c.blocks = (uint32_t)(blocks < most ? blocks : most);
+    return c;
+}
+
 template <int DT, int D, int GS>
 cudaError_t run_append(const Rows& k, const Rows& v, const void* slots, int wide, const Kv4Cache& c, uint32_t tokens, bool vec, unsigned* err, cudaStream_t s) {
-    constexpr uint32_t per_block = 8u * (D < 128 ? 128 / D : 1);
-    const uint64_t units = (uint64_t)tokens * c.kv_heads * (D < 128 ? 1 : D / 128);
-    uint64_t blocks = (units + per_block - 1) / per_block;
-    const uint64_t most = (uint64_t)device_sms() * 8u;
-    if (blocks > most) blocks = most;
-    return launch_early(vec ? append_kernel<DT, D, GS, true> : append_kernel<DT, D, GS, false>, dim3((unsigned)blocks), dim3(256), 0, s, k, v, slots, wide, c,
-                        tokens, err);
+    const Cut cut = cut_heads(tokens, c.kv_heads, D);
+    return launch_early(vec ? append_kernel<DT, D, GS, true> : append_kernel<DT, D, GS, false>, dim3(cut.blocks), dim3(256), 0, s, k, v, slots, wide, c, tokens,
+                        cut.chunks, cut.rounds, err);
 }
 
 template <int DT, int D, int GS>
 cudaError_t run_gather(const Kv4Cache& c, const void* slots, int wide, void* k, void* v, uint32_t tokens, unsigned* err, cudaStream_t s) {
-    uint64_t blocks = ((uint64_t)tokens * c.kv_heads * (D / 4) + 255u) / 256u;
-    const uint64_t most = (uint64_t)device_sms() * 16u;
-    if (blocks > most) blocks = most;
-    return launch_early(gather_kernel<DT, D, GS>, dim3((unsigned)blocks), dim3(256), 0, s, c, slots, wide, k, v, tokens, err);
+    const Cut cut = cut_heads(tokens, c.kv_heads, D);
+    return launch_early(gather_kernel<DT, D, GS>, dim3(cut.blocks), dim3(256), 0, s, c, slots, wide, k, v, tokens, cut.chunks, cut.rounds, err);
 }
 
 // f.template operator()<DT, D, GS>() for the types, heads and groups that the cache takes
@@ -440,15 +536,19 @@ cudaError_t launch_rotary(int dt, const Rows& q, uint32_t q_heads, const Rows& k
     int vec = (r / 2u) % W == 0 && (d - r) % (2 * W) == 0;
     for (const Rows* x : {&q, &k, &qo, &ko})
         if (x->p) vec &= aligned(x->p, x->token, x->head, W, size);
-    // a token is one block while there are tokens enough for every SM; fewer are cut by heads
+    // several tokens to a block while there are blocks enough for every SM; where there are few tokens, they are cut by heads
     const uint32_t steps = (q_heads + k_heads) * d / (2u * (vec ? W : 1));
-    uint32_t cut = (2u * device_sms() + tokens - 1u) / tokens;
-    const uint32_t most = (steps + 255u) / 256u;
-    if (cut > most) cut = most;
-    if (cut == 0) cut = 1;
-    const dim3 grid(tokens, cut);
-#define ROTARY(DT_) return interleaved ? rotary_any<DT_, false>(vec, grid, s, q, q_heads, k, k_heads, qo, ko, positions, wide, f, tokens, d, r, factor) \
-                                       : rotary_any<DT_, true>(vec, grid, s, q, q_heads, k, k_heads, qo, ko, positions, wide, f, tokens, d, r, factor)
+    uint32_t span = 1, cut = 1;
+    while (span < 4u && tokens / (2u * span) >= 8u * device_sms() && 2u * span * r / 2u <= 2u * kMaxRotaryPairs) span *= 2u;
+    if (span == 1u) {
+        cut = (2u * device_sms() + tokens - 1u) / tokens;
+        const uint32_t most = (steps + 255u) / 256u;
+        if (cut > most) cut = most;
+        if (cut == 0) cut = 1;
+    }
+    const dim3 grid((tokens + span - 1u) / span, cut);
+#define ROTARY(DT_) return interleaved ? rotary_any<DT_, false>(vec, grid, span, s, q, q_heads, k, k_heads, qo, ko, positions, wide, f, tokens, d, r, factor) \
+                                       : rotary_any<DT_, true>(vec, grid, span, s, q, q_heads, k, k_heads, qo, ko, positions, wide, f, tokens, d, r, factor)
     if (dt == FP32) ROTARY(FP32);
     if (dt == FP16) ROTARY(FP16);
     ROTARY(BF16);

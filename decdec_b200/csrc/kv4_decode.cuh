@@ -129,8 +129,13 @@ template <int D, int GS, int NT> __host__ __device__ constexpr size_t decode_sme
     return ring > merge ? ring : merge;
 }
 
+// blocks of an SM that the registers are cut for: as many as need no spills worth the name
+template <int D, int GS, int NT> __host__ __device__ constexpr int decode_residency() {
+    return D == 256 ? 2 : NT == 1 ? (D / GS <= 2 ? 4 : 3) : D == 64 ? 3 : 2;
+}
+
 template <int D, int GS, int NT, int DT>
-__global__ void __launch_bounds__(kDecodeThreads) kv4_decode_kernel(Kv4Attn p) {
+__global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>()) kv4_decode_kernel(Kv4Attn p) {
     using T = typename Tr<DT>::T;
     using Sh = DecodeShape<D, NT>;
     constexpr int NG = D / GS;                  // groups of a head
