@@ -23,8 +23,6 @@
 #pragma once
 #include "kv4.cuh"
 
-#include <type_traits>
-
 namespace dd {
 
 constexpr int kDecodeThreads = 128;
@@ -38,7 +36,7 @@ __host__ __device__ constexpr uint32_t kv4_part_floats(uint32_t d, uint32_t nt) 
 // how many parts, and of which segment, the block that began a cut segment leaves behind
 struct Kv4Cut {
     uint32_t parts;                    // 0: this block cut no segment that it began
-    uint32_t request, row0, head;      // row0: first row of the tile among the request's rows
+    uint32_t row0, head;               // row0: first row of the tile among the request's rows
     uint32_t start, rows;              // first token of the request among all, rows of the request
 };
 
@@ -76,6 +74,21 @@ __device__ __forceinline__ void code_pairs(uint32_t x, uint32_t (&h)[4]) {
     }
 }
 
+// the codes of a word as fp16 pairs 1024 + 16 code: (0, 4), (1, 5), (2, 6), (3, 7).  Two instructions a pair less than above; the 1024 is
+// taken out of the sums over a head, which costs them 2^-21 of their terms.
+__device__ __forceinline__ void raised_pairs(uint32_t x, uint32_t (&h)[4]) {
+    const __half2 by = __float2half2_rn(16.0f), less = __float2half2_rn(-15360.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t y = i < 2 ? x : x >> 8;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(h[i]) : "r"(y), "r"(i & 1 ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
+        if (!(i & 1)) {
+            const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&h[i]), by, less);       // 16 (1024 + code) - 15 * 1024
+            h[i] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+    }
+}
+
 // N consecutive 32-bit words of shared memory, in the widest loads
 template <int N> __device__ __forceinline__ void load_words(uint32_t (&x)[N], const uint8_t* at) {
     if constexpr (N % 4 == 0) {
@@ -90,6 +103,11 @@ template <int N> __device__ __forceinline__ void load_words(uint32_t (&x)[N], co
     } else {
         x[0] = *reinterpret_cast<const uint32_t*>(at);
     }
+}
+
+// quotient of numbers that almost always fit 32 bits, where a division costs a fifth
+__device__ __forceinline__ unsigned long long ratio_of(unsigned long long a, unsigned long long b) {
+    return ((a | b) >> 32) == 0 ? (unsigned long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 // what a request asks for
@@ -121,17 +139,16 @@ template <int D, int NT> struct DecodeShape {
     static constexpr int kRowStride = D + 4;            // floats; keeps the warps' 16-byte stores apart by banks
     static constexpr int kMergeFloats = kDecodeWarps * kRows * (kRowStride + 2);
 };
-// A step of a warp is two neighbouring cells (32 tokens), and kStages steps of a warp lie in shared memory.  The warps' sums are added in
-// the same memory once a segment's steps are through.
+// A step of a warp is two neighbouring cells (32 tokens), and kStages steps of a warp lie in shared memory, beside the place where the
+// warps' sums are added: the next segment's first steps are under way meanwhile.
 constexpr int kStages = 3;
 template <int D, int GS, int NT> __host__ __device__ constexpr size_t decode_smem() {
-    const size_t ring = (size_t)kDecodeWarps * kStages * 2u * kv4_cell_bytes(D, GS), merge = DecodeShape<D, NT>::kMergeFloats * 4u;
-    return ring > merge ? ring : merge;
+    return (size_t)kDecodeWarps * kStages * 2u * kv4_cell_bytes(D, GS) + DecodeShape<D, NT>::kMergeFloats * 4u;
 }
 
 // blocks of an SM that the registers are cut for: as many as need no spills worth the name
 template <int D, int GS, int NT> __host__ __device__ constexpr int decode_residency() {
-    return D == 256 ? 2 : NT == 1 ? (D / GS <= 2 ? 4 : 3) : D == 64 ? 3 : 2;
+    return D == 256 ? 2 : NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 : 2;
 }
 
 template <int D, int GS, int NT, int DT>
@@ -150,7 +167,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     const int gid = lane >> 2, tig = lane & 3;
     uint8_t* ring = smem + (size_t)warp * kStages * 2 * CELL;
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-    float* merge = reinterpret_cast<float*>(smem);                                            // [warp][row][kRowStride]
+    float* merge = reinterpret_cast<float*>(smem + (size_t)kDecodeWarps * kStages * 2 * CELL);   // [warp][row][kRowStride]
     float* merge_ml = merge + kDecodeWarps * Sh::kRows * Sh::kRowStride;                      // [warp][row][2]
     uint8_t* after = reinterpret_cast<uint8_t*>(p.part + (size_t)gridDim.x * 2u * kv4_part_floats(D, NT));
     Kv4Cut* cuts = reinterpret_cast<Kv4Cut*>(after);
@@ -181,7 +198,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
         total += s_sum[w];
     }
     // at least two cells a warp: a shorter part would spend its time in the joining of the parts
-    const long long per = max((total + gridDim.x - 1) / gridDim.x, 2ll * kDecodeWarps);
+    const long long per = max((long long)ratio_of(total + gridDim.x - 1, gridDim.x), 2ll * kDecodeWarps);
     const long long x0 = (long long)blockIdx.x * per, x1 = min(x0 + per, total);
     const long long excl = before + incl - mine;
     if (x0 < x1 && excl <= x0 && x0 < excl + mine) {
@@ -210,13 +227,48 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     if (x0 < x1) {
         uint32_t b = s_request;
         Kv4Request rq = kv4_request(p, b, Sh::kRows, false);
-        long long rest = s_rest;
-        int item = (int)(rest / rq.cells);                   // tile * kv_heads + head
-        int c0 = (int)(rest % rq.cells);
+        int item = (int)ratio_of(s_rest, rq.cells);          // tile * kv_heads + head
+        int c0 = (int)(s_rest - (long long)item * rq.cells), c1 = (int)min((long long)rq.cells, c0 + (x1 - x0));
+        uint32_t head = (uint32_t)item % p.kv_heads;
         long long x = x0;
+
+        // ---- this warp's steps of a segment: cells c0 + 2 (warp + 4 j), + 1
+        int count;
+        uint32_t cell_at, fill;                              // place in the cache of the cell 2 j + lane of its steps; stage that is filled next
+        auto places_of = [&](int j0) {
+            const int c = rq.first + c0 + 2 * (warp + kDecodeWarps * (j0 + (lane >> 1))) + (lane & 1);
+            cell_at = kNoCell;
+            if (c < rq.first + c1 && c * kCellTokens < rq.length) {
+                const uint32_t column = (uint32_t)c / p.page_cells;
+                const int page = p.table[(long long)b * p.table_stride + column];
+                if (page >= 0 && (uint32_t)page < p.pages) cell_at = ((uint32_t)page * p.kv_heads + head) * p.page_cells + (uint32_t)c % p.page_cells;
+                else raise_error(p.err, kErrKv4Page);
+            }
+        };
+        auto issue = [&](int j) {
+            if (j < count) {
+                if ((j & 15) == 0) places_of(j);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t at = __shfl_sync(0xffffffffu, cell_at, 2 * (j & 15) + u);
+                    const uint32_t bytes = at == kNoCell ? 0u : 16u;       // zeros, from a source that is not read
+                    const uint8_t* src = p.cache + (size_t)(at == kNoCell ? 0u : at) * CELL + lane * 16u;
+#pragma unroll
+                    for (uint32_t i = 0; i < (CELL / 16 + 31) / 32; ++i)
+                        if (CELL % 512 == 0 || i * 512u + lane * 16u < CELL) cp_async16(fill + u * CELL + i * 512u, src + i * 512u, bytes);
+                }
+                fill = fill == ring_s + lane * 16u + (kStages - 1) * 2u * CELL ? ring_s + lane * 16u : fill + 2u * CELL;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        auto begin = [&] {
+            count = ((c1 - c0 + 1) / 2 - warp + kDecodeWarps - 1) / kDecodeWarps;
+            fill = ring_s + lane * 16u;
+#pragma unroll
+            for (int j = 0; j < kStages - 1; ++j) issue(j);
+        };
+        begin();
         while (x < x1) {
-            const int c1 = (int)min((long long)rq.cells, c0 + (x1 - x));
-            const uint32_t head = (uint32_t)item % p.kv_heads;
             const int row0 = (int)((uint32_t)item / p.kv_heads) * Sh::kRows;
             const int all_rows = rq.queries * (int)p.ratio;
 
@@ -289,7 +341,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
             }
             // tokens that each of this lane's rows sees: [from, to)
             int from[NT][2], to[NT][2];
-            const int pos0 = rq.length - rq.queries, end = (rq.first + c1) * kCellTokens;      // the segment's cells end there
+            const int pos0 = rq.length - rq.queries, end = (rq.first + c1) * kCellTokens;        // the segment's cells end there
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -303,7 +355,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
             const int first_pos = pos0 + row0 / (int)p.ratio, last_pos = pos0 + (min(row0 + Sh::kRows, all_rows) - 1) / (int)p.ratio;
             const int clear_to = min(max(first_pos + 1, 0), end), clear_from = p.window ? (int)max(0ll, (long long)last_pos - (long long)p.window + 1) : 0;
 
-            float acc[D / 16][NT][4], off[NT][2][NG], l[NT][2], m[NT][2];
+            float acc[D / 16][NT][4], off[NT][2][NG], l[NT][2], m[NT][2], less[NT][2];
             float fv[NG], limit[NG];                         // factor of the steps, and the step that it is good for
 #pragma unroll
             for (int i = 0; i < D / 16; ++i)
@@ -321,41 +373,10 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) { l[nt][i] = 0.0f; m[nt][i] = -INFINITY; }
+                for (int i = 0; i < 2; ++i) { l[nt][i] = 0.0f; m[nt][i] = -INFINITY; less[nt][i] = 0.0f; }
 
-            // ---- this warp's steps: cells c0 + 2 (warp + 4 j), + 1
-            const int count = ((c1 - c0 + 1) / 2 - warp + kDecodeWarps - 1) / kDecodeWarps;
-            uint32_t cell_at = kNoCell;                      // place in the cache of the cell 2 j0 + lane of this warp's steps
-            auto places_of = [&](int j0) {
-                const int c = rq.first + c0 + 2 * (warp + kDecodeWarps * (j0 + (lane >> 1))) + (lane & 1);
-                cell_at = kNoCell;
-                if (c < rq.first + c1 && c * kCellTokens < rq.length) {
-                    const uint32_t column = (uint32_t)c / p.page_cells;
-                    const int page = p.table[(long long)b * p.table_stride + column];
-                    if (page >= 0 && (uint32_t)page < p.pages) cell_at = ((uint32_t)page * p.kv_heads + head) * p.page_cells + (uint32_t)c % p.page_cells;
-                    else raise_error(p.err, kErrKv4Page);
-                }
-            };
-            uint32_t fill = ring_s + lane * 16u;
-            auto issue = [&](int j) {
-                if (j < count) {
-                    if ((j & 15) == 0) places_of(j);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t at = __shfl_sync(0xffffffffu, cell_at, 2 * (j & 15) + u);
-                        const uint32_t bytes = at == kNoCell ? 0u : 16u;       // zeros, from a source that is not read
-                        const uint8_t* src = p.cache + (size_t)(at == kNoCell ? 0u : at) * CELL + lane * 16u;
-#pragma unroll
-                        for (uint32_t i = 0; i < (CELL / 16 + 31) / 32; ++i)
-                            if (CELL % 512 == 0 || i * 512u + lane * 16u < CELL) cp_async16(fill + u * CELL + i * 512u, src + i * 512u, bytes);
-                    }
-                    fill = fill == ring_s + lane * 16u + (kStages - 1) * 2u * CELL ? ring_s + lane * 16u : fill + 2u * CELL;
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            // One step.  CLEAR: every row of the tile sees all 32 tokens.
-            auto step = [&](const uint8_t* st, int tok0, auto clear_tag) {
-                constexpr bool CLEAR = decltype(clear_tag)::value;
+            // One step.  clear: every row of the tile sees all 32 tokens.
+            auto step = [&](const uint8_t* st, int tok0, bool clear) {
                 constexpr int PER = NW < 4 ? NW : 4;          // words of a lane in a block
                 constexpr int VB = D < 128 ? 1 : D / 128, VP = NW / VB;      // blocks of values, words of a lane and plane in each
                 // ---- scores: rows = tokens gid, gid + 8 of cell u; columns = queries 2 tig, 2 tig + 1
@@ -369,10 +390,14 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                     for (int i = 0; i < 2; ++i) {
                         load_words(kr[i], cell + kv4_key_step(D, GS, gid + 8 * i, 0));
                         load_words(vr[u][i], cell + kv4_value_step(D, GS, gid + 8 * i, 0));
-                        if (!CLEAR && tok0 + 16 * u + 8 * i + gid >= rq.length) {      // behind the end lies what the page held before
+                    }
+                    if (!clear) {
 #pragma unroll
-                            for (int g = 0; g < NG; ++g) kr[i][g] = vr[u][i][g] = 0u;
-                        }
+                        for (int i = 0; i < 2; ++i)
+                            if (tok0 + 16 * u + 8 * i + gid >= rq.length) {            // behind the end lies what the page held before
+#pragma unroll
+                                for (int g = 0; g < NG; ++g) kr[i][g] = vr[u][i][g] = 0u;
+                            }
                     }
                     uint32_t xa[NW / PER][PER], xb[NW / PER][PER];
 #pragma unroll
@@ -390,8 +415,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
 #pragma unroll
                         for (int w = g * GS / 32; w < (g + 1) * GS / 32; ++w) {
                             uint32_t ca[4], cb[4];
-                            code_pairs(xa[w / PER][w % PER], ca);
-                            code_pairs(xb[w / PER][w % PER], cb);
+                            raised_pairs(xa[w / PER][w % PER], ca);
+                            raised_pairs(xb[w / PER][w % PER], cb);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
                                 mma_16816<FP16>(raw[nt], ca[0], cb[0], ca[1], cb[1], qf[nt][w][0], qf[nt][w][1]);
@@ -402,8 +427,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const float2 f = unpack2<DT>(kr[i][g]);
-                            ks[i] = f.x;
-                            ko[i] = fmaf(8.0f, f.x, f.y);
+                            ks[i] = 0.0625f * f.x;
+                            ko[i] = fmaf(-64.0f, f.x, f.y);            // offset less the 1024 / 16 steps that the codes are raised by
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
@@ -414,19 +439,33 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                             }
                     }
                 }
-                bool follow = false;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s[u][nt][i] *= sf[nt][i & 1];
-                            if (!CLEAR) {
+                        for (int i = 0; i < 4; ++i) s[u][nt][i] *= sf[nt][i & 1];
+                bool poison = false;                          // a token that some row does not see holds no number: its product with 0 counts
+                if (!clear) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
                                 const int tok = tok0 + 16 * u + gid + 8 * (i >> 1);
                                 if (tok < from[nt][i & 1] || tok >= to[nt][i & 1]) s[u][nt][i] = -INFINITY;
                             }
-                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) poison |= !(fabsf(unpack2<DT>(vr[u][i][g]).y) < INFINITY);
+                    }
+                    poison = __any_sync(0xffffffffu, poison);
+                }
+                bool follow = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
                         follow |= fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i])) > m[nt][i] + kGrow;
@@ -449,6 +488,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                             top = fmaxf(top, m[nt][i]);
                             down[nt][i] = top == m[nt][i] ? 1.0f : ex2(m[nt][i] - top);
                             m[nt][i] = top;
+                            less[nt][i] = top == -INFINITY ? 0.0f : top;      // a row that has seen nothing yet: its weights are 0
                             l[nt][i] *= down[nt][i];
                         }
 #pragma unroll
@@ -483,8 +523,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            // a row that has seen nothing yet has the maximum -inf: its weights are 0
-                            w[nt][i] = (!CLEAR && s[u][nt][i] == -INFINITY) ? 0.0f : ex2(s[u][nt][i] - m[nt][i & 1]);
+                            w[nt][i] = ex2(s[u][nt][i] - less[nt][i & 1]);
                             l[nt][i & 1] += w[nt][i];
                         }
                     // ---- outputs: rows = elements, depth = tokens, columns = queries; planes of tokens 0..7 and 8..15
@@ -502,11 +541,12 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                         for (int nt = 0; nt < NT; ++nt) {
                             b0[nt] = movmatrix(half2_bits(w[nt][0] * f0, w[nt][1] * f0));
                             b1[nt] = movmatrix(half2_bits(w[nt][2] * f1, w[nt][3] * f1));
+                            if (!poison) {
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                if (CLEAR) {
-                                    off[nt][i][g] = fmaf(w[nt][i], o0, fmaf(w[nt][2 + i], o1, off[nt][i][g]));
-                                } else {                     // a token that this row does not see may hold no number
+                                for (int i = 0; i < 2; ++i) off[nt][i][g] = fmaf(w[nt][i], o0, fmaf(w[nt][2 + i], o1, off[nt][i][g]));
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
                                     off[nt][i][g] += w[nt][i] == 0.0f ? 0.0f : w[nt][i] * o0;
                                     off[nt][i][g] += w[nt][2 + i] == 0.0f ? 0.0f : w[nt][2 + i] * o1;
                                 }
@@ -526,8 +566,6 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                     }
                 }
             };
-#pragma unroll
-            for (int j = 0; j < kStages - 1; ++j) issue(j);
             const uint8_t* st = ring;
             int tok0 = (rq.first + c0 + 2 * warp) * kCellTokens;
             for (int j = 0; j < count; ++j) {
@@ -535,13 +573,32 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 __syncwarp();
                 issue(j + kStages - 1);                      // into the stage that the last step read
                 // behind the end of the segment's cells lies another block's work: `to` hides it
-                if (tok0 >= clear_from && tok0 + 2 * kCellTokens <= clear_to) step(st, tok0, std::true_type{});
-                else step(st, tok0, std::false_type{});
+                step(st, tok0, tok0 >= clear_from && tok0 + 2 * kCellTokens <= clear_to);
                 st = st == ring + (kStages - 1) * 2 * CELL ? ring : st + 2 * CELL;
                 tok0 += kDecodeWarps * 2 * kCellTokens;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            __syncthreads();                                 // every warp is through with its ring
+            __syncwarp();                                    // the warp is through with its ring
+
+            // ---- on to the next segment, whose first steps travel while this one's sums are added
+            const bool whole = c0 == 0 && c1 == rq.cells, late = c0 > 0;
+            const int start = rq.start;
+            const uint32_t at_head = head;
+            if (!whole && !late) {                           // it ends in block (x + cells - 1) / per
+                cut.parts = (uint32_t)(ratio_of(x + rq.cells - 1, per) - blockIdx.x) + 1u;
+                cut.row0 = (uint32_t)row0; cut.head = head; cut.start = (uint32_t)start; cut.rows = (uint32_t)all_rows;
+            }
+            x += c1 - c0;
+            if (x < x1) {
+                if (++item == rq.tiles * (int)p.kv_heads) {
+                    item = 0;
+                    do rq = kv4_request(p, ++b, Sh::kRows, false); while (rq.tiles == 0);      // ends: cells remain
+                }
+                c0 = 0;
+                c1 = (int)min((long long)rq.cells, x1 - x);
+                head = (uint32_t)item % p.kv_heads;
+                begin();
+            }
 
             // ---- the warps' sums into shared memory
 #pragma unroll
@@ -573,8 +630,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                     }
                 }
             __syncthreads();
-            const bool whole = c0 == 0 && c1 == rq.cells;
-            float* part = p.part + ((size_t)blockIdx.x * 2u + (c0 > 0 ? 0u : 1u)) * kv4_part_floats(D, NT);
+            float* part = p.part + ((size_t)blockIdx.x * 2u + (late ? 0u : 1u)) * kv4_part_floats(D, NT);
             for (int e = tid; e < Sh::kRows * (D / 4); e += kDecodeThreads) {
                 const int r = e / (D / 4), d4 = e % (D / 4);
                 float top = -INFINITY, mw[kDecodeWarps];
@@ -597,7 +653,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 if (whole) {
                     if (row < all_rows) {
                         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                        const long long tok = rq.start + row / (int)p.ratio, h = head * p.ratio + row % (int)p.ratio;
+                        const long long tok = start + row / (int)p.ratio, h = at_head * p.ratio + row % (int)p.ratio;
                         T* dst = reinterpret_cast<T*>(p.out) + tok * p.out_token + h * p.out_head + 4 * d4;
                         T o[4] = {Tr<DT>::from_f(v.x * inv), Tr<DT>::from_f(v.y * inv), Tr<DT>::from_f(v.z * inv), Tr<DT>::from_f(v.w * inv)};
                         *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
@@ -612,17 +668,6 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 }
             }
             __syncthreads();
-            if (!whole && c0 == 0) {
-                // the segment ends in block (x + cells - 1) / per
-                cut.parts = (uint32_t)((x + rq.cells - 1) / per - blockIdx.x) + 1u;
-                cut.request = b; cut.row0 = (uint32_t)row0; cut.head = head; cut.start = (uint32_t)rq.start; cut.rows = (uint32_t)all_rows;
-            }
-            x += c1 - c0;
-            c0 = 0;
-            if (x < x1 && ++item == rq.tiles * (int)p.kv_heads) {
-                item = 0;
-                do rq = kv4_request(p, ++b, Sh::kRows, false); while (rq.tiles == 0);      // ends: cells remain
-            }
         }
     }
     if (tid == 0) cuts[blockIdx.x] = cut;
@@ -635,62 +680,47 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(Kv4Attn p, uint32_t block
     constexpr int LANES = D / 4;                     // threads across a row
     constexpr int WAYS = 128 / LANES;                // parts taken at the same time
     __shared__ float4 s_v[WAYS][LANES];
-    __shared__ float s_ml[128][2];
-    __shared__ float s_all[2];
+    __shared__ float s_ml[WAYS][2];
     pdl_trigger();
     pdl_wait();
     const Kv4Cut cut = reinterpret_cast<const Kv4Cut*>(p.part + (size_t)blocks * 2u * kv4_part_floats(D, NT))[blockIdx.x];
     const uint32_t r = blockIdx.y, row = cut.row0 + r;
     if (cut.parts == 0 || row >= cut.rows) return;
     const float* base = p.part + (size_t)blockIdx.x * 2u * kv4_part_floats(D, NT);
-    // part 0 is this block's second, part i the first of block + i
-    auto part = [&](uint32_t i) { return base + (size_t)(i == 0 ? 1u : 2u * i) * kv4_part_floats(D, NT); };
-    const uint32_t tid = threadIdx.x;
-    float m = -INFINITY, l = 0.0f;
-    for (uint32_t i = tid; i < cut.parts; i += 128u) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(i) + 8 * NT * D + 2 * r));
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-        const float top = fmaxf(m, ml.x);
-        l = l * (m == top ? 1.0f : ex2(m - top)) + ml.y * (ml.x == top ? 1.0f : ex2(ml.x - top));
-        m = top;
-    }
-    s_ml[tid][0] = m;
-    s_ml[tid][1] = l;
-    __syncthreads();
-    if (tid < 32) {
-        for (int i = 1; i < 4; ++i) {
-            const float m2 = s_ml[tid + 32 * i][0], top = fmaxf(m, m2);
-            l = l * (m == top ? 1.0f : ex2(m - top)) + s_ml[tid + 32 * i][1] * (m2 == top ? 1.0f : ex2(m2 - top));
-            m = top;
+    const uint32_t way = threadIdx.x / LANES, d4 = threadIdx.x % LANES;
+    float top = -INFINITY, sum = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float m, float l, const float4& o) {
+        if (m == -INFINITY && l == 0.0f) return;                          // saw nothing
+        const float to = fmaxf(top, m), f0 = top == to ? 1.0f : ex2(top - to), f1 = m == to ? 1.0f : ex2(m - to);
+        top = to;
+        sum = sum * f0 + l * f1;
+        v.x = v.x * f0 + o.x * f1; v.y = v.y * f0 + o.y * f1; v.z = v.z * f0 + o.z * f1; v.w = v.w * f0 + o.w * f1;
+    };
+    constexpr uint32_t U = 8;                                             // parts that a thread has under way
+    for (uint32_t i0 = way; i0 < cut.parts; i0 += WAYS * U) {
+        float2 ml[U];
+        float4 o[U];
+#pragma unroll
+        for (uint32_t k = 0; k < U; ++k) {
+            const uint32_t i = i0 + WAYS * k;
+            ml[k] = make_float2(-INFINITY, 0.0f);
+            if (i < cut.parts) {
+                // part 0 is this block's second, part i the first of block + i
+                const float* at = base + (size_t)(i == 0 ? 1u : 2u * i) * kv4_part_floats(D, NT);
+                ml[k] = __ldcg(reinterpret_cast<const float2*>(at + 8 * NT * D + 2 * r));
+                o[k] = __ldcg(reinterpret_cast<const float4*>(at + r * D + 4 * d4));
+            }
         }
 #pragma unroll
-        for (int o = 16; o; o /= 2) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o), top = fmaxf(m, m2);
-            l = l * (m == top ? 1.0f : ex2(m - top)) + l2 * (m2 == top ? 1.0f : ex2(m2 - top));
-            m = top;
-        }
-        if (tid == 0) { s_all[0] = m; s_all[1] = l; }
-    }
-    __syncthreads();
-    const float top = s_all[0], sum = s_all[1];
-    const uint32_t way = tid / LANES, d4 = tid % LANES;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (uint32_t i = way; i < cut.parts; i += WAYS) {
-        const float* at = part(i);
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(at + 8 * NT * D + 2 * r));
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(at + r * D + 4 * d4));
-        const float f = (ml.x == -INFINITY && ml.y == 0.0f) ? 0.0f : ml.x == top ? 1.0f : ex2(ml.x - top);
-        v.x = fmaf(o.x, f, v.x); v.y = fmaf(o.y, f, v.y); v.z = fmaf(o.z, f, v.z); v.w = fmaf(o.w, f, v.w);
+        for (uint32_t k = 0; k < U; ++k) add(ml[k].x, ml[k].y, o[k]);
     }
     s_v[way][d4] = v;
+    if (d4 == 0) { s_ml[way][0] = top; s_ml[way][1] = sum; }
     __syncthreads();
     if (way == 0) {
 #pragma unroll
-        for (int w = 1; w < WAYS; ++w) {
-            const float4 o = s_v[w][d4];
-            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-        }
+        for (int w = 1; w < WAYS; ++w) add(s_ml[w][0], s_ml[w][1], s_v[w][d4]);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const long long tok = cut.start + row / p.ratio, h = cut.head * p.ratio + row % p.ratio;
         T* dst = reinterpret_cast<T*>(p.out) + tok * p.out_token + h * p.out_head + 4 * d4;
