@@ -22,7 +22,7 @@ LIB = PKG / "libdecdec_b200.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = ["host.cu", "k_dec.cu", "k_bcq.cu", "k_anyprec.cu", "k_sqllm.cu", "noalloc.cu", "tp_allreduce.cu",
-              "k_kv4.cu", "k_kv4_attn.cu", "k_kv4_decode64.cu", "k_kv4_decode128.cu", "k_kv4_decode256.cu"]
+              "k_kv4.cu", "k_kv4_attn.cu", "k_kv4_decode64.cu", "k_kv4_decode128.cu", "k_kv4_decode256.cu", "k_kv4_chunk.cu"]
 
 
 def _run(cmd, log=None):

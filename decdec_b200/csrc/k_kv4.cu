@@ -208,10 +208,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Plan p) {
 }
 
 // ---- rows into the cache -----------------------------------------------------------------------------------
-template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    typename Tr<DT>::T v[2] = {Tr<DT>::from_f(a), Tr<DT>::from_f(b)};
-    return *reinterpret_cast<const uint32_t*>(v);
-}
 template <int DT> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
     if constexpr (DT == FP16) {
         const __half2 r = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));

@@ -2,6 +2,7 @@
 #include "internal.h"
 #include "kv4.cuh"
 #include "kv4_decode.cuh"
+#include "kv4_chunk.cuh"
 #include "../../include/decdec_b200.h"
 
 #include <cmath>
@@ -16,18 +17,29 @@ int fail(int code, const char* fmt, unsigned long long a = 0, unsigned long long
     return set_last_error(code, msg);
 }
 
-// tiles of 8 rows while the requests' rows fit one, of 16 else; heads of 256 elements have no registers for 16
-uint32_t row_tiles(uint32_t head_dim, uint32_t ratio, uint32_t max_queries) {
-    return head_dim <= 128 && (uint64_t)ratio * max_queries > 8 ? 2 : 1;
-}
+// Which kernel, and how many blocks fill the device.
+struct Choice {
+    bool chunk;                 // tiles of 256 rows on the fifth-generation tensor cores
+    uint32_t nt;                // else tiles of 8 nt rows
+    uint32_t blocks;
+    size_t bytes;               // of the workspace
+};
 
-int blocks_per_sm(uint32_t head_dim, uint32_t group, uint32_t nt, int dt) {
-    return head_dim == 64 ? kv4_decode64_blocks_per_sm(group, nt, dt) : head_dim == 128 ? kv4_decode128_blocks_per_sm(group, nt, dt)
-                                                                                        : kv4_decode256_blocks_per_sm(group, nt, dt);
-}
-
-size_t decode_bytes(uint32_t head_dim, uint32_t nt, uint32_t blocks) {
-    return (size_t)blocks * (2u * kv4_part_floats(head_dim, nt) * sizeof(float) + sizeof(Kv4Cut));
+// Tiles of 8 rows while a request's rows (queries x heads of a key head) fit one, of 16 while they fit two; heads of 256 elements have no
+// registers for 16 and no room for 256.
+int choose(uint32_t head_dim, uint32_t group, uint32_t ratio, uint32_t max_queries, int dt, Choice* c) {
+    const uint64_t rows = (uint64_t)ratio * max_queries;
+    c->chunk = head_dim <= 128 && ratio <= (uint32_t)kChunkRows && rows > 16;
+    c->nt = c->chunk ? kChunkRows / 8 : head_dim <= 128 && rows > 8 ? 2 : 1;
+    c->blocks = device_sms();
+    if (!c->chunk) {
+        const int per_sm = head_dim == 64 ? kv4_decode64_blocks_per_sm(group, c->nt, dt) : head_dim == 128 ? kv4_decode128_blocks_per_sm(group, c->nt, dt)
+                                                                                                           : kv4_decode256_blocks_per_sm(group, c->nt, dt);
+        if (per_sm < 1) return fail(DECDEC_E_CUDA, "the attention kernel does not fit the current device");
+        c->blocks *= (uint32_t)per_sm;
+    }
+    c->bytes = (size_t)c->blocks * (2u * kv4_part_floats(head_dim, c->nt) * sizeof(float) + sizeof(Kv4Cut));
+    return 0;
 }
 
 int check(uint32_t requests, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t group, uint32_t max_queries, int dtype) {
@@ -52,10 +64,9 @@ int decdec_kv4_attention_workspace(uint32_t requests, uint32_t rows, uint32_t he
                                    uint32_t max_queries, int dtype, size_t* bytes) {
     if (!bytes) return fail(DECDEC_E_INVALID, "null output pointer");
     if (int r = check(requests, rows, heads, kv_heads, head_dim, group_size, max_queries, dtype)) return r;
-    const uint32_t nt = row_tiles(head_dim, heads / kv_heads, max_queries);
-    const int per_sm = blocks_per_sm(head_dim, group_size, nt, dtype);
-    if (per_sm < 1) return fail(DECDEC_E_CUDA, "the decode attention kernel does not fit the current device");
-    *bytes = decode_bytes(head_dim, nt, device_sms() * (uint32_t)per_sm);
+    Choice c;
+    if (int r = choose(head_dim, group_size, heads / kv_heads, max_queries, dtype, &c)) return r;
+    *bytes = c.bytes;
     return 0;
 }
 
@@ -75,11 +86,10 @@ int decdec_kv4_attention(const void* q, int64_t q_token, int64_t q_head, void* o
     if (!q || !out || !cache || (requests && (!lengths || !query_starts)) || (requests && table_cols && !table)) return fail(DECDEC_E_INVALID, "null pointer argument");
     if (reinterpret_cast<uintptr_t>(cache) & 15u) return fail(DECDEC_E_INVALID, "the cache must be 16-byte aligned device memory");
     if ((reinterpret_cast<uintptr_t>(out) & 7u) || out_token % 4 || out_head % 4) return fail(DECDEC_E_INVALID, "output rows must be 8-byte aligned");
-    const uint32_t ratio = heads / kv_heads, nt = row_tiles(head_dim, ratio, max_queries);
-    const int per_sm = blocks_per_sm(head_dim, group_size, nt, dtype);
-    if (per_sm < 1) return fail(DECDEC_E_CUDA, "the decode attention kernel does not fit the current device");
-    const uint32_t most = device_sms() * (uint32_t)per_sm;
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < decode_bytes(head_dim, nt, most))
+    const uint32_t ratio = heads / kv_heads;
+    Choice c;
+    if (int r = choose(head_dim, group_size, ratio, max_queries, dtype, &c)) return r;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < c.bytes)
         return fail(DECDEC_E_INVALID, "workspace must be 16-byte aligned and hold what decdec_kv4_attention_workspace says");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     Kv4Attn p = {};
@@ -97,15 +107,20 @@ int decdec_kv4_attention(const void* q, int64_t q_token, int64_t q_head, void* o
     p.q_vec = (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && q_token % 8 == 0 && q_head % 8 == 0;
     p.fill_tail = clear_tail ? 1u : 0u;
     p.scale_log2 = scale * 1.4426950408889634f;
-    // no more blocks than the longest contexts that the table holds could give two cells a warp
-    const uint64_t tiles = ((uint64_t)rows * ratio + 8u * nt - 1) / (8u * nt) + requests;
-    const uint64_t cells = tiles * kv_heads * ((uint64_t)table_cols * p.page_cells + 1u);
-    uint64_t blocks = (cells + 2 * kDecodeWarps - 1) / (2 * kDecodeWarps);
-    if (blocks > most) blocks = most;
-    if (blocks == 0) blocks = 1;
-    cudaError_t e = head_dim == 64    ? launch_kv4_decode64(group_size, nt, dtype, p, (uint32_t)blocks, s)
-                    : head_dim == 128 ? launch_kv4_decode128(group_size, nt, dtype, p, (uint32_t)blocks, s)
-                                      : launch_kv4_decode256(group_size, nt, dtype, p, (uint32_t)blocks, s);
+    cudaError_t e;
+    if (c.chunk) {
+        e = launch_kv4_chunk(head_dim, group_size, dtype, p, c.blocks, s);
+    } else {
+        // no more blocks than the longest contexts that the table holds could give two cells a warp
+        const uint64_t tiles = ((uint64_t)rows * ratio + 8u * c.nt - 1) / (8u * c.nt) + requests;
+        const uint64_t cells = tiles * kv_heads * ((uint64_t)table_cols * p.page_cells + 1u);
+        uint64_t blocks = (cells + 2 * kDecodeWarps - 1) / (2 * kDecodeWarps);
+        if (blocks > c.blocks) blocks = c.blocks;
+        if (blocks == 0) blocks = 1;
+        e = head_dim == 64    ? launch_kv4_decode64(group_size, c.nt, dtype, p, (uint32_t)blocks, s)
+            : head_dim == 128 ? launch_kv4_decode128(group_size, c.nt, dtype, p, (uint32_t)blocks, s)
+                              : launch_kv4_decode256(group_size, c.nt, dtype, p, (uint32_t)blocks, s);
+    }
     if (e != cudaSuccess) {
         char msg[256];
         snprintf(msg, sizeof(msg), "attention launch failed: %s", cudaGetErrorString(e));

@@ -41,6 +41,11 @@ __host__ __device__ constexpr uint32_t kv4_value_step(uint32_t d, uint32_t group
     return 16u * d + 64u * (d / group) + (r * (d / group) + g) * 4u;
 }
 
+template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typename Tr<DT>::T v[2] = {Tr<DT>::from_f(a), Tr<DT>::from_f(b)};
+    return *reinterpret_cast<const uint32_t*>(v);
+}
+
 // rows [tokens][heads][head_dim] of a 16-bit type, strides in elements
 struct Rows {
     const void* p;
@@ -86,6 +91,9 @@ KV4_DECODE(64);
 KV4_DECODE(128);
 KV4_DECODE(256);
 #undef KV4_DECODE
+
+// Attention of many queries, heads of 64 and 128: one block an SM
+cudaError_t launch_kv4_chunk(uint32_t head_dim, uint32_t group, int dt, const Kv4Attn& p, uint32_t blocks, cudaStream_t s);
 
 // A launch whose blocks may become resident while the previous kernel of the stream drains (every kernel here waits for it before
 // it reads anything); DECDEC_PDL=0 turns that off.

@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     if (tid == 0) cuts[blockIdx.x] = cut;
 }
 
-// Adds the parts of a cut segment: one block per (block that began one, row of the tile).
+// Adds the parts of a cut segment: blocks (block that began one, row of the tile modulo gridDim.y).
 template <int D, int NT, int DT>
 __global__ void __launch_bounds__(128) kv4_join_kernel(Kv4Attn p, uint32_t blocks) {
     using T = typename Tr<DT>::T;
@@ -684,49 +684,52 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(Kv4Attn p, uint32_t block
     pdl_trigger();
     pdl_wait();
     const Kv4Cut cut = reinterpret_cast<const Kv4Cut*>(p.part + (size_t)blocks * 2u * kv4_part_floats(D, NT))[blockIdx.x];
-    const uint32_t r = blockIdx.y, row = cut.row0 + r;
-    if (cut.parts == 0 || row >= cut.rows) return;
+    if (cut.parts == 0) return;
     const float* base = p.part + (size_t)blockIdx.x * 2u * kv4_part_floats(D, NT);
     const uint32_t way = threadIdx.x / LANES, d4 = threadIdx.x % LANES;
-    float top = -INFINITY, sum = 0.0f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float m, float l, const float4& o) {
-        if (m == -INFINITY && l == 0.0f) return;                          // saw nothing
-        const float to = fmaxf(top, m), f0 = top == to ? 1.0f : ex2(top - to), f1 = m == to ? 1.0f : ex2(m - to);
-        top = to;
-        sum = sum * f0 + l * f1;
-        v.x = v.x * f0 + o.x * f1; v.y = v.y * f0 + o.y * f1; v.z = v.z * f0 + o.z * f1; v.w = v.w * f0 + o.w * f1;
-    };
-    constexpr uint32_t U = 8;                                             // parts that a thread has under way
-    for (uint32_t i0 = way; i0 < cut.parts; i0 += WAYS * U) {
-        float2 ml[U];
-        float4 o[U];
+    for (uint32_t r = blockIdx.y; r < 8 * NT && cut.row0 + r < cut.rows; r += gridDim.y) {
+        const uint32_t row = cut.row0 + r;
+        float top = -INFINITY, sum = 0.0f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float m, float l, const float4& o) {
+            if (m == -INFINITY && l == 0.0f) return;                          // saw nothing
+            const float to = fmaxf(top, m), f0 = top == to ? 1.0f : ex2(top - to), f1 = m == to ? 1.0f : ex2(m - to);
+            top = to;
+            sum = sum * f0 + l * f1;
+            v.x = v.x * f0 + o.x * f1; v.y = v.y * f0 + o.y * f1; v.z = v.z * f0 + o.z * f1; v.w = v.w * f0 + o.w * f1;
+        };
+        constexpr uint32_t U = 8;                                             // parts that a thread has under way
+        for (uint32_t i0 = way; i0 < cut.parts; i0 += WAYS * U) {
+            float2 ml[U];
+            float4 o[U];
 #pragma unroll
-        for (uint32_t k = 0; k < U; ++k) {
-            const uint32_t i = i0 + WAYS * k;
-            ml[k] = make_float2(-INFINITY, 0.0f);
-            if (i < cut.parts) {
-                // part 0 is this block's second, part i the first of block + i
-                const float* at = base + (size_t)(i == 0 ? 1u : 2u * i) * kv4_part_floats(D, NT);
-                ml[k] = __ldcg(reinterpret_cast<const float2*>(at + 8 * NT * D + 2 * r));
-                o[k] = __ldcg(reinterpret_cast<const float4*>(at + r * D + 4 * d4));
+            for (uint32_t k = 0; k < U; ++k) {
+                const uint32_t i = i0 + WAYS * k;
+                ml[k] = make_float2(-INFINITY, 0.0f);
+                if (i < cut.parts) {
+                    // part 0 is this block's second, part i the first of block + i
+                    const float* at = base + (size_t)(i == 0 ? 1u : 2u * i) * kv4_part_floats(D, NT);
+                    ml[k] = __ldcg(reinterpret_cast<const float2*>(at + 8 * NT * D + 2 * r));
+                    o[k] = __ldcg(reinterpret_cast<const float4*>(at + r * D + 4 * d4));
+                }
             }
+#pragma unroll
+            for (uint32_t k = 0; k < U; ++k) add(ml[k].x, ml[k].y, o[k]);
         }
+        s_v[way][d4] = v;
+        if (d4 == 0) { s_ml[way][0] = top; s_ml[way][1] = sum; }
+        __syncthreads();
+        if (way == 0) {
 #pragma unroll
-        for (uint32_t k = 0; k < U; ++k) add(ml[k].x, ml[k].y, o[k]);
-    }
-    s_v[way][d4] = v;
-    if (d4 == 0) { s_ml[way][0] = top; s_ml[way][1] = sum; }
-    __syncthreads();
-    if (way == 0) {
-#pragma unroll
-        for (int w = 1; w < WAYS; ++w) add(s_ml[w][0], s_ml[w][1], s_v[w][d4]);
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const long long tok = cut.start + row / p.ratio, h = cut.head * p.ratio + row % p.ratio;
-        T* dst = reinterpret_cast<T*>(p.out) + tok * p.out_token + h * p.out_head + 4 * d4;
-        T o[4] = {Tr<DT>::from_f(v.x * inv), Tr<DT>::from_f(v.y * inv), Tr<DT>::from_f(v.z * inv), Tr<DT>::from_f(v.w * inv)};
-        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
-        if (p.lse && d4 == 0) p.lse[(size_t)tok * p.kv_heads * p.ratio + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+            for (int w = 1; w < WAYS; ++w) add(s_ml[w][0], s_ml[w][1], s_v[w][d4]);
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const long long tok = cut.start + row / p.ratio, h = cut.head * p.ratio + row % p.ratio;
+            T* dst = reinterpret_cast<T*>(p.out) + tok * p.out_token + h * p.out_head + 4 * d4;
+            T o[4] = {Tr<DT>::from_f(v.x * inv), Tr<DT>::from_f(v.y * inv), Tr<DT>::from_f(v.z * inv), Tr<DT>::from_f(v.w * inv)};
+            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+            if (p.lse && d4 == 0) p.lse[(size_t)tok * p.kv_heads * p.ratio + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+        }
+        __syncthreads();                                                  // the sums in shared memory are the next row's
     }
 }
 

@@ -82,26 +82,31 @@ def rotary(x, positions, frequencies, interleaved, factor):
     return y
 
 
-def attention(q, k, v, length, scale, window, group):
-    """One request: q [n, heads, D], k, v [length, kv_heads, D] as given to append.  Returns out, bound of the error, lse (64 bits).
+def attention(q, k, v, length, scale, window, group, dense=False):
+    """One request: q [n, heads, D], k, v [length, kv_heads, D] as given to append.  Returns out, bound of its error, lse, bound of a score's rounding
+    (64 bits).
 
     The bound counts, per output: half a step of the output's type; half an fp16 step (2^-11) of every product weight * step, times
     |code - 8|; 2^-10 for what bounded scores do to the weights (2^-20 of the sum of |q| |k| per score, twice) and for sums in 32 bits;
-    weights that become subnormal, 2^-28 of the largest each."""
+    weights that become subnormal, 2^-28 of the largest each.
+    dense: for many queries keys and values are rounded to fp16 on the way, middle and result (2^-11 each): a score is then off by 2^-10 of the
+    sum of |q| (|k| + |middle|), a weight by twice that relative to the others, and the values count for 2^-10 more."""
     n, heads, d = q.shape
     kv_heads = k.shape[1]
     ratio = heads // kv_heads
     out = torch.zeros(n, heads, d, dtype=torch.float64)
     bound = torch.zeros_like(out)
     lse = torch.full((n, heads), -math.inf, dtype=torch.float64)
+    score_bound = torch.zeros((), dtype=torch.float64)
     if n == 0 or length == 0:
-        return out, bound, lse
+        return out, bound, lse, score_bound
     pos = torch.arange(length - n, length)[:, None]
     tok = torch.arange(length)
     seen = tok <= pos
     if window:
         seen &= tok > pos - window
     kd = held(k[:length], group)
+    _, kstep, klo = quantize(k[:length], group)
     code, step, lo = quantize(v[:length], group)
     vd = held(v[:length], group)
     away = (step[..., None] * (code.unflatten(-1, (-1, group)) - 8).abs()).flatten(-2)
@@ -121,7 +126,13 @@ def attention(q, k, v, length, scale, window, group):
         a, w = p @ away[:, g].nan_to_num(0.0), p @ whole[:, g].nan_to_num(0.0)
         bound[:, h] = HALF[q.dtype] * (out[:, h].abs() + w * 2.0 ** -9) + 2.0 ** -11 * a + (2.0 ** -10 * 2.0 ** -4 + 2.0 ** -19 * worst) * w + \
             length * 2.0 ** -28 * whole[:, g].nan_to_num(0.0).amax(0) + 1e-30
-    return out, bound, lse
+        if dense:
+            middle = klo + 8 * kstep
+            size = kd.abs() + middle.abs().repeat_interleave(group, -1)
+            off = torch.where(seen, 2.0 ** -10 * q[:, h].double().abs() @ size[:, g].T * scale, 0.0).nan_to_num(0.0).amax(-1, keepdim=True)
+            score_bound = torch.maximum(score_bound, off.max())
+            bound[:, h] += (2.0 ** -10 + torch.expm1(2 * off)) * w + 2.0 ** -11 * w
+    return out, bound, lse, score_bound
 
 
 def pages_of(lengths, page_size, extra, seed):

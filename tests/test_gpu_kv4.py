@@ -275,13 +275,16 @@ class Batch:
 
     def run(self, q=None, **kw):
         q = self.q.cuda() if q is None else q
+        # the rule that the kernel is chosen by: more than 16 rows (queries x heads of a key head) of a request, heads up to 128
+        rows = min(kw.get("max_queries", len(q)), len(q)) * (q.shape[1] // self.cache.shape[1])
+        self.dense = rows > 16 and self.d <= 128 and q.shape[1] // self.cache.shape[1] <= 256
         return self.kv4.attention(q, self.cache, self.table.cuda(), torch.tensor(self.lengths, dtype=torch.int32).cuda(), self.starts.cuda(), self.group, **kw)
 
     def check(self, out, lse=None, scale=None, window=0):
         scale = self.d ** -0.5 if scale is None else scale
         at = 0
         for b, n in enumerate(self.queries):
-            want, bound, want_lse = R.attention(self.q[at:at + n], self.k[b], self.v[b], self.lengths[b], scale, window, self.group)
+            want, bound, want_lse, by = R.attention(self.q[at:at + n], self.k[b], self.v[b], self.lengths[b], scale, window, self.group, self.dense)
             got = out[at:at + n].cpu().double()
             assert torch.equal(torch.isnan(got), torch.isnan(want)), b
             off = ((got - want).abs() - bound).nan_to_num(0.0)
@@ -290,7 +293,7 @@ class Batch:
                 l = lse[at:at + n].cpu().double()
                 inf = torch.isinf(want_lse)
                 assert torch.equal(inf, torch.isinf(l))
-                assert ((l - want_lse)[~inf].abs() <= 2e-5 * (1 + want_lse[~inf].abs())).all()
+                assert ((l - want_lse)[~inf].abs() <= 2e-5 * (1 + want_lse[~inf].abs()) + by).all()
             at += n
 
 
@@ -312,6 +315,19 @@ def test_attention_several_queries(kv4, dtype, window, d, group, heads, kv_heads
     b = Batch(kv4, lengths, queries, heads, kv_heads, d, group, dtype, page, 200)
     out, lse = b.run(window=window, return_lse=True, scale=0.2)
     b.check(out, lse, window=window, scale=0.2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group", FORMATS[:5])
+@pytest.mark.parametrize("heads,kv_heads,window", [(4, 4, 0), (8, 2, 0), (5, 1, 0), (8, 2, 100), (33, 1, 300)])
+def test_attention_of_chunks(kv4, dtype, d, group, heads, kv_heads, window):
+    """Tiles of rows and steps of 128 tokens that end anywhere, requests with one query among them."""
+    lengths, queries = [129, 1, 400, 128, 300, 17], [129, 1, 70, 5, 1, 17]
+    b = Batch(kv4, lengths, queries, heads, kv_heads, d, group, dtype, 16, 250)
+    out, lse = b.run(window=window, return_lse=True)
+    assert b.dense
+    b.check(out, lse, window=window)
+    assert torch.equal(out, b.run(window=window))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -424,7 +440,7 @@ def test_cache_beyond_32_bit_offsets(kv4):
     gk, _ = kv4.gather(cache, slots.cuda(), d, group, torch.float16)
     assert ((gk.cpu().double() - R.held(k, group)).abs() <= 2.0 ** -10 * 1.01 * k.double().abs().amax()).all()
     out = kv4.attention(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda(), group)
-    want, bound, _ = R.attention(q, k, v, n, d ** -0.5, 0, group)
+    want, bound, _, _ = R.attention(q, k, v, n, d ** -0.5, 0, group)
     assert ((out.cpu().double() - want).abs() <= bound).all()
 
 
@@ -525,7 +541,8 @@ def test_steps_of_a_layer(kv4, dtype, d, group, interleaved):
             assert ((got_k.double() - want_k).abs() <= R.HALF[dtype] * want_k.abs() + 1e-5).all()
             kept_k[b].append(got_k)
             kept_v[b].append(v[at:at + m].cpu())
-            want, bound, _ = R.attention(result["q"][at:at + m].cpu(), torch.cat(kept_k[b]), torch.cat(kept_v[b]), before[b] + m, d ** -0.5, 0, group)
+            want, bound, _, _ = R.attention(result["q"][at:at + m].cpu(), torch.cat(kept_k[b]), torch.cat(kept_v[b]), before[b] + m, d ** -0.5, 0, group,
+                                             max(new) * heads // kv_heads > 16)
             assert ((result["out"][at:at + m].cpu().double() - want).abs() <= bound).all()
             at += m
         assert (result["out"][n:] == 0).all()
