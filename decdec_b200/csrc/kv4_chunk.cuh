@@ -93,11 +93,11 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t (&r)[32]) {
                  : "r"(at));
 }
 __device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(at));
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                   "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -561,78 +561,65 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                     const ChunkMeta& meta = s_meta[step & 3u];
                     const int tok0 = (g.t.from + g.c0 + j) * kChunkStep;
                     const bool clear = tok0 >= clear_from && tok0 + kChunkStep <= clear_to;
-                    const int4 key_exp = *reinterpret_cast<const int4*>(meta.key_exp), value_exp = *reinterpret_cast<const int4*>(meta.value_exp);
-                    const int ke[4] = {key_exp.x, key_exp.y, key_exp.z, key_exp.w}, ve[4] = {value_exp.x, value_exp.y, value_exp.z, value_exp.w};
-                    int new_ev = max(max(ve[0], ve[1]), max(ve[2], ve[3]));
+                    const int4 ve = *reinterpret_cast<const int4*>(meta.value_exp);
+                    int new_ev = max(max(ve.x, ve.y), max(ve.z, ve.w));
                     if (j > 0) new_ev = max(new_ev, ev);
-                    // tokens 16 c .. of the step that the row sees
-                    auto seen = [&](int c) {
-                        const int lo = max(from - (tok0 + 16 * c), 0), hi = min(to - (tok0 + 16 * c), 16);
-                        return lo >= hi ? 0u : (0xffffffffu >> (32 - (hi - lo))) << lo;
-                    };
-                    uint32_t r[2][16];
-                    tmem_load16(at_s, r[0]);
-                    // sums, and the weights of the step that are written already, brought to another maximum or exponent
-                    auto bring = [&](float by, int written) {
-                        if (j > 0) {
+                    // 32 tokens at a time, in a loop that is not unrolled: the roles' code has to stay in the instruction cache
 #pragma unroll 1
-                            for (int c = 0; c < D / 8; ++c) {
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t r[32];
+                        tmem_load32(at_s + 32 * c, r);
+                        const float f = sf * pow2(meta.key_exp[c] - 12);
+                        // weights times 2^(exponent of the values here - that of the sums)
+                        const int shift = max(meta.value_exp[c] - new_ev, -126);
+                        tmem_loaded();
+                        if (!clear) {
+                            const int lo = max(from - (tok0 + 32 * c), 0), hi = min(to - (tok0 + 32 * c), 32);
+                            const uint32_t mask = lo >= hi ? 0u : (0xffffffffu >> (32 - (hi - lo))) << lo;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (!((mask >> i) & 1u)) r[i] = 0xff800000u;             // -inf: a weight of 0
+                        }
+                        float top = __uint_as_float(r[0]);
+#pragma unroll
+                        for (int i = 1; i < 32; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+                        top *= f;
+                        const bool follow = top > m + kChunkGrow || (c == 0 && j > 0 && new_ev != ev);
+                        if (__any_sync(0xffffffffu, follow)) {
+                            // rare after a segment's first steps: the sums, and the weights of the step that are written already, brought to
+                            // another maximum or exponent
+                            const float now = fmaxf(m, top), down = m == now ? 1.0f : ex2(m - now), by = down * ex2((float)((j > 0 && c == 0 ? ev : new_ev) - new_ev));
+                            m = now;
+                            l *= down;
+                            tmem_stored();
+                            for (int k = 0; j > 0 && k < D / 8; ++k) {
                                 uint32_t o[8];
-                                tmem_load8(at_o + 8 * c, o);
+                                tmem_load8(at_o + 8 * k, o);
                                 tmem_loaded();
 #pragma unroll
                                 for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
-                                tmem_store8(at_o + 8 * c, o);
+                                tmem_store8(at_o + 8 * k, o);
+                            }
+                            const __half2 h = __float2half2_rn(down);
+                            for (int k = 0; k < 2 * c; ++k) {
+                                uint32_t o[8];
+                                tmem_load8(at_s + 8 * k, o);
+                                tmem_loaded();
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&o[i]), h);
+                                    o[i] = *reinterpret_cast<const uint32_t*>(&x);
+                                }
+                                tmem_store8(at_s + 8 * k, o);
                             }
                         }
-#pragma unroll 1
-                        for (int c = 0; c < written; ++c) {
-                            uint32_t o[8];
-                            tmem_stored();
-                            tmem_load8(at_s + 8 * c, o);
-                            tmem_loaded();
-                            const __half2 h = __float2half2_rn(by);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&o[i]), h);
-                                o[i] = *reinterpret_cast<const uint32_t*>(&x);
-                            }
-                            tmem_store8(at_s + 8 * c, o);
-                        }
-                    };
-                    if (j > 0 && new_ev != ev) bring(ex2((float)(ev - new_ev)), 0);      // the same for all rows
-                    ev = new_ev;
-                    float less = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const float f = sf * pow2(ke[c / 2] - 12);
-                        const uint32_t mask = clear ? 0u : seen(c);
-                        tmem_loaded();
-                        if (c < 7) tmem_load16(at_s + 16 * (c + 1), r[(c + 1) & 1]);
-                        float top = -INFINITY;
-                        if (!clear) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (!((mask >> i) & 1u)) r[c & 1][i] = 0xff800000u;      // -inf: a weight of 0
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) top = fmaxf(top, __uint_as_float(r[c & 1][i]));
-                        top *= f;
-                        if (__any_sync(0xffffffffu, top > m + kChunkGrow)) {             // rare after a segment's first steps
-                            const float now = fmaxf(m, top), down = m == now ? 1.0f : ex2(m - now);
-                            m = now;
-                            less = m == -INFINITY ? 0.0f : m;
-                            l *= down;
-                            bring(down, c);
-                        }
-                        // weights times 2^(exponent of the values here - that of the sums)
-                        const int shift = max(ve[c / 2] - ev, -126);
-                        const unsigned long long by = pair_of(f, f), off = pair_of((float)shift - less, (float)shift - less);
+                        const float less = (float)shift - (m == -INFINITY ? 0.0f : m);
+                        const unsigned long long by = pair_of(f, f), off = pair_of(less, less);
                         unsigned long long sum = 0ull;
-                        uint32_t w[8];
+                        uint32_t w[16];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float2 x = of_pair(fma_pair(pair_of(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), by, off));
+                        for (int i = 0; i < 16; ++i) {
+                            float2 x = of_pair(fma_pair(pair_of(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), by, off));
                             x.x = ex2(x.x);
                             x.y = ex2(x.y);
                             sum = add_pair(sum, pair_of(x.x, x.y));
@@ -640,8 +627,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                         }
                         const float2 part = of_pair(sum);
                         l = fmaf(part.x + part.y, pow2(-shift), l);
-                        tmem_store8(at_s + 8 * c, w);
+                        tmem_store16(at_s + 16 * c, w);
                     }
+                    ev = new_ev;
                     tmem_stored();
                     const uint4 any = *reinterpret_cast<const uint4*>(meta.any_poison);
                     const uint32_t marked = any.x | any.y | any.z | any.w;
