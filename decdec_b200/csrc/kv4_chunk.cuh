@@ -509,11 +509,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
             const int live_rows = g.t.n * (int)p.ratio, steps = g.c1 - g.c0;
             const bool active = grp == 0 || live_rows > 128, live = row < live_rows;
             const int query = g.t.q0 + (live ? row / (int)p.ratio : 0), sub = live ? row % (int)p.ratio : 0;
-            const long long tok = g.r.start + query, qh = (long long)g.head * p.ratio + sub;
             float sf;
             {
                 // the row as fp16, scaled to a power of two near 2^13; read twice, to hold little of it
-                const T* src = reinterpret_cast<const T*>(p.q.p) + tok * p.q.token + qh * p.q.head;
+                const T* src = reinterpret_cast<const T*>(p.q.p) + (long long)(g.r.start + query) * p.q.token + ((long long)g.head * p.ratio + sub) * p.q.head;
                 auto eight = [&](int c) {
                     if (!live) return make_uint4(0, 0, 0, 0);
                     if (p.q_vec) return *reinterpret_cast<const uint4*>(src + 8 * c);
@@ -631,26 +630,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                     }
                     ev = new_ev;
                     tmem_stored();
-                    const uint4 any = *reinterpret_cast<const uint4*>(meta.any_poison);
-                    const uint32_t marked = any.x | any.y | any.z | any.w;
-                    if (marked) {
-                        for (int i = 0; i < NG; ++i)
-                            for (int c = 0; c < 4; ++c)
-                                for (uint32_t bits = meta.poison[i][c]; bits; bits &= bits - 1u) {
-                                    const int at = tok0 + 32 * c + __ffs(bits) - 1;
-                                    if (at >= from && at < to) bad |= 1u << i;
-                                }
-                    }
                 }
                 tc_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar_p + 8 * grp);
+                const ChunkMeta& meta = s_meta[step & 3u];
+                const uint4 any = *reinterpret_cast<const uint4*>(meta.any_poison);
+                if (any.x | any.y | any.z | any.w) {
+                    const int tok0 = (g.t.from + g.c0 + j) * kChunkStep;
+                    for (int i = 0; i < NG; ++i)
+                        for (int c = 0; c < 4; ++c)
+                            for (uint32_t bits = meta.poison[i][c]; bits; bits &= bits - 1u) {
+                                const int at = tok0 + 32 * c + __ffs(bits) - 1;
+                                if (at >= from && at < to) bad |= 1u << i;
+                            }
+                }
             }
             bar_wait(bar_o, seg & 1u, gave_up, p.err);
             ++seg;
             tc_after();
             const bool whole = g.c0 == 0 && g.c1 == g.t.steps, late = g.c0 > 0;
             if (active && any_live) {
+                const long long tok = g.r.start + query, qh = (long long)g.head * p.ratio + sub;
                 float* part = p.part + ((size_t)blockIdx.x * 2u + (late ? 0u : 1u)) * kv4_part_floats(D, kChunkRows / 8);
                 const float unit = pow2(min(max(ev - 12, -126), 127)), by = whole ? (l == 0.0f ? 0.0f : unit / l) : unit;
                 T* dst = reinterpret_cast<T*>(p.out) + tok * p.out_token + qh * p.out_head;

@@ -275,9 +275,9 @@ class Batch:
 
     def run(self, q=None, **kw):
         q = self.q.cuda() if q is None else q
-        # the rule that the kernel is chosen by: more than 16 rows (queries x heads of a key head) of a request, heads up to 128
+        # the rule that the kernel is chosen by: more than 64 rows (queries x heads of a key head) of a request, heads up to 128
         rows = min(kw.get("max_queries", len(q)), len(q)) * (q.shape[1] // self.cache.shape[1])
-        self.dense = rows > 16 and self.d <= 128 and q.shape[1] // self.cache.shape[1] <= 256
+        self.dense = rows > 64 and self.d <= 128 and q.shape[1] // self.cache.shape[1] <= 256
         return self.kv4.attention(q, self.cache, self.table.cuda(), torch.tensor(self.lengths, dtype=torch.int32).cuda(), self.starts.cuda(), self.group, **kw)
 
     def check(self, out, lse=None, scale=None, window=0):
@@ -542,7 +542,7 @@ def test_steps_of_a_layer(kv4, dtype, d, group, interleaved):
             kept_k[b].append(got_k)
             kept_v[b].append(v[at:at + m].cpu())
             want, bound, _, _ = R.attention(result["q"][at:at + m].cpu(), torch.cat(kept_k[b]), torch.cat(kept_v[b]), before[b] + m, d ** -0.5, 0, group,
-                                             max(new) * heads // kv_heads > 16)
+                                             max(new) * heads // kv_heads > 64)
             assert ((result["out"][at:at + m].cpu().double() - want).abs() <= bound).all()
             at += m
         assert (result["out"][n:] == 0).all()
