@@ -208,15 +208,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Plan p) {
 }
 
 // ---- rows into the cache -----------------------------------------------------------------------------------
-template <int DT> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
-    if constexpr (DT == FP16) {
-        const __half2 r = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-        return *reinterpret_cast<const uint32_t*>(&r);
-    } else {
-        const __nv_bfloat162 r = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-}
+// a register of two 16-bit values
+template <int DT> struct Two;
+template <> struct Two<FP16> { using T = __half2; };
+template <> struct Two<BF16> { using T = __nv_bfloat162; };
+template <int DT> __device__ __forceinline__ typename Two<DT>::T as2(uint32_t v) { return *reinterpret_cast<const typename Two<DT>::T*>(&v); }
+template <int DT> __device__ __forceinline__ uint32_t bits2(typename Two<DT>::T v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// the smaller of each, NaN if one is
+template <int DT> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) { return bits2<DT>(__hmin2_nan(as2<DT>(a), as2<DT>(b))); }
 // whether one of the two 16-bit values is infinite or NaN
 template <int DT> __device__ __forceinline__ uint32_t no_number(uint32_t v) {
     constexpr uint32_t E = DT == FP16 ? 0x7c007c00u : 0x7f807f80u, U = DT == FP16 ? 0x04000400u : 0x00800080u;
@@ -248,32 +247,40 @@ template <int DT> __device__ __forceinline__ float step_of(float lo, float hi) {
     return Tr<DT>::to_f(Tr<DT>::from_f(q));
 }
 
-// four codes of 16-bit values a, b in a 16-bit word
-template <int DT> __device__ __forceinline__ uint32_t code_word(uint32_t a, uint32_t b, float lo, float step) {
+// eight codes of 16-bit values in a word
+template <int DT> __device__ __forceinline__ uint32_t code_word(const uint4& x, float lo, float step) {
     if (!(step > 0.0f)) return 0u;
-    const float2 fa = unpack2<DT>(a), fb = unpack2<DT>(b);
-    const float h[4] = {0.5f * fa.x, 0.5f * fa.y, 0.5f * fb.x, 0.5f * fb.y};
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
     const float loh = 0.5f * lo, steph = 0.5f * step;
     const bool small = steph < 1e-30f;                           // its reciprocal may overflow
     float inv;                                                   // a guess: what it is off by stays far below `near`
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(steph));
     if (small) inv = 0.0f;
     const float near = steph * 0.4999f;
+    // a normal step is off by 2^-8 at most, so no quotient comes near 15.5; a subnormal one may be off by half of it
+    bool border = step < (DT == FP16 ? 6.103515625e-5f : 1.17549435e-38f) || small;
     uint32_t word = 0;
-    bool border = small;
-    float n[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float d = h[j] - loh;
-        const float up = fmaf(d, inv, 12582912.0f);              // 1.5 * 2^23: the sum's last bits are the rounded quotient
-        n[j] = up - 12582912.0f;
-        border |= fabsf(fmaf(-n[j], steph, d)) > near || n[j] > 15.0f;       // next to a border; beyond the last code (subnormal steps)
-        word |= (__float_as_uint(up) & 15u) << (4 * j);
+    for (int i = 0; i < 2; ++i) {
+        float four = 0.0f;                                       // the codes as digits, which 24 bits hold
+#pragma unroll
+        for (int k = 3; k >= 0; --k) {
+            const float2 f = unpack2<DT>(u[2 * i + k / 2]);
+            const float d = fmaf(0.5f, k & 1 ? f.y : f.x, -loh); // the product is exact
+            const float n = fmaf(d, inv, 12582912.0f) - 12582912.0f;         // 1.5 * 2^23: the sum is rounded to a whole number
+            border |= fabsf(fmaf(-n, steph, d)) > near;          // next to a border
+            four = fmaf(four, 16.0f, n);
+        }
+        word |= (__float_as_uint(four + 8388608.0f) & 0xffffu) << (16 * i);
     }
-    if (border) {                                                // of the four, about one in 2^10 random ones; more in short types
+    if (border) {                                                // of the eight, about one in 2^9 random ones; more in short types
         word = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) word |= (uint32_t)exact_code(h[j], loh, steph, small ? rintf((h[j] - loh) / steph) : n[j]) << (4 * j);
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = unpack2<DT>(u[i / 2]);
+            const float h = 0.5f * (i & 1 ? f.y : f.x), d = h - loh;
+            word |= (uint32_t)exact_code(h, loh, steph, small ? rintf(d / steph) : rintf(d * inv)) << (4 * i);
+        }
     }
     return word;
 }
@@ -297,138 +304,152 @@ __device__ __forceinline__ Place place_of(const Kv4Cache& c, const void* slots, 
     return p;
 }
 
-// A warp takes a token and `rounds` warps' widths of its heads; a lane the four elements of a 16-bit word of keys and of values, so 128
-// elements of a head are one coalesced 256-byte read of each, and the group extremes are a few shuffles of (least, -largest) pairs.  Bound
-// by the instructions, about 15 an element: the slot is looked up once for all heads, ties are settled apart.
+// How a warp lies on a token: eight elements a lane, so 8 or 16 lanes on a head (128 of its elements if there are 256), the keys of all
+// heads of a round on the first half of the warp and their values on the second.
+template <int D> struct Lanes {
+    static constexpr uint32_t kBlock = D < 128 ? D : 128;           // elements of a unit
+    static constexpr uint32_t kUnit = kBlock / 8;                   // lanes of a unit
+    static constexpr uint32_t kUnits = D / kBlock;                  // units of a head
+    static constexpr uint32_t kRound = 16 / kUnit;                  // units of a round, keys and values
+};
+
+constexpr uint32_t kRounds = 4;                                     // of a warp at most
+
+// A warp takes a token and `rounds` rounds of its heads, which are coalesced 256-byte reads of keys and values; the group extremes are a
+// few shuffles of (least, -largest) pairs.  Bound by the instructions, about 9 an element: the slot is looked up once for all heads, ties
+// are settled apart.  8191 tokens of 10 heads of 128: four elements a lane 26 us, eight 20.
 template <int DT, int D, int GS, bool VEC>
 __global__ void __launch_bounds__(256) append_kernel(Rows k, Rows v, const void* slots, int wide, Kv4Cache c, uint32_t tokens, uint32_t chunks, uint32_t rounds,
                                                      unsigned* err) {
     using T = typename Tr<DT>::T;
-    constexpr uint32_t BL = D < 128 ? D : 128;          // elements of a unit
-    constexpr uint32_t LANES = BL / 4;                   // lanes of a unit
-    constexpr uint32_t UNITS = D / BL;                   // units of a head
-    constexpr uint32_t PER_WARP = 32 / LANES;
-    constexpr int GL = GS / 4;                           // lanes of a group
+    using L = Lanes<D>;
+    constexpr int GL = GS / 8;                           // lanes of a group
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31u, all = c.kv_heads * UNITS;
+    const uint32_t lane = threadIdx.x & 31u, all = c.kv_heads * L::kUnits;
+    const bool side = lane >= 16u;
+    const Rows& x = side ? v : k;
     const uint64_t items = (uint64_t)tokens * chunks;
     for (uint64_t i = (uint64_t)blockIdx.x * (blockDim.x / 32u) + (threadIdx.x >> 5); i < items; i += (uint64_t)gridDim.x * (blockDim.x / 32u)) {
         const uint32_t t = quotient(i, chunks), chunk = (uint32_t)(i - (uint64_t)t * chunks);
         const Place at = place_of(c, slots, wide, t, kv4_cell_bytes(D, GS), lane == 0u && chunk == 0u, err);
         if (!at.inside) continue;
-        const uint32_t first = chunk * rounds * PER_WARP + lane / LANES;
-#pragma unroll 2
-        for (uint32_t round = 0; round < rounds; ++round) {
-            const uint32_t unit = first + round * PER_WARP;
-            const bool live = unit < all;
-            const uint32_t h = live ? unit / UNITS : 0u, u = unit % UNITS * (BL / 4) + lane % LANES;
-            uint32_t raw[2][2] = {{0, 0}, {0, 0}};
-            if (live) {
+        const T* row = reinterpret_cast<const T*>(x.p) + (long long)t * x.token;
+        const uint32_t first = chunk * rounds * L::kRound + (lane & 15u) / L::kUnit;
+        uint4 all_raw[kRounds];
 #pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                    const Rows& x = side ? v : k;
-                    const T* src = reinterpret_cast<const T*>(x.p) + (long long)t * x.token + (long long)h * x.head + 4u * u;
-                    if constexpr (VEC) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(src);
-                        raw[side][0] = w.x; raw[side][1] = w.y;
-                    } else {
-                        const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
-                        raw[side][0] = (uint32_t)e[0] | (uint32_t)e[1] << 16;
-                        raw[side][1] = (uint32_t)e[2] | (uint32_t)e[3] << 16;
-                    }
+        for (uint32_t round = 0; round < kRounds; ++round) {         // everything that the warp reads is under way at once
+            const uint32_t unit = first + round * L::kRound;
+            all_raw[round] = make_uint4(0, 0, 0, 0);
+            if (round < rounds && unit < all) {
+                const T* src = row + (long long)(unit / L::kUnits) * x.head + unit % L::kUnits * L::kBlock + lane % L::kUnit * 8u;
+                if constexpr (VEC) {
+                    all_raw[round] = *reinterpret_cast<const uint4*>(src);
+                } else {
+                    const uint16_t* w = reinterpret_cast<const uint16_t*>(src);
+                    all_raw[round] = make_uint4((uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16,
+                                                (uint32_t)w[4] | (uint32_t)w[5] << 16, (uint32_t)w[6] | (uint32_t)w[7] << 16);
                 }
             }
-            uint8_t* cell = at.cell + (size_t)h * c.page_bytes;
+        }
 #pragma unroll
-            for (int side = 0; side < 2; ++side) {
-                const uint32_t a = raw[side][0], b = raw[side][1];
-                // (least, -largest): a minimum over both signs, then over the lanes of the group; an element that is no number makes the
-                // range infinite, and the group reads back as NaN
-                const uint32_t low = min2<DT>(a, b), high = min2<DT>(a ^ 0x80008000u, b ^ 0x80008000u);
-                uint32_t range = min2<DT>(__byte_perm(low, high, 0x5410), __byte_perm(low, high, 0x7632));
-                if (no_number<DT>(a) | no_number<DT>(b)) range = DT == FP16 ? 0xfc00fc00u : 0xff80ff80u;
+        for (uint32_t round = 0; round < kRounds; ++round) {
+            if (round >= rounds) break;
+            const uint32_t unit = first + round * L::kRound;
+            const bool live = unit < all;
+            const uint32_t h = live ? unit / L::kUnits : 0u, e = unit % L::kUnits * L::kBlock + lane % L::kUnit * 8u;
+            const uint4 raw = all_raw[round];
+            // (least, -largest): a minimum over both signs, then over the lanes of the group.  One that is no number comes through, and the
+            // group reads back as NaN
+            const uint32_t s = 0x80008000u;
+            const uint32_t low = min2<DT>(min2<DT>(raw.x, raw.y), min2<DT>(raw.z, raw.w));
+            const uint32_t high = min2<DT>(min2<DT>(raw.x ^ s, raw.y ^ s), min2<DT>(raw.z ^ s, raw.w ^ s));
+            uint32_t range = min2<DT>(__byte_perm(low, high, 0x5410), __byte_perm(low, high, 0x7632));
 #pragma unroll
-                for (int o = 1; o < GL; o *= 2) range = min2<DT>(range, __shfl_xor_sync(0xffffffffu, range, o));
-                const float2 lh = unpack2<DT>(range);
-                float lo = lh.x, step = step_of<DT>(lo, -lh.y);
-                if (lo == -INFINITY) { lo = __int_as_float(0x7fc00000); step = 0.0f; }
-                const uint32_t word = code_word<DT>(a, b, lo, step);
-                if (live) {
-                    *reinterpret_cast<uint16_t*>(cell + (side ? kv4_value_word(D, at.r, u) : kv4_key_word(D, at.r, u))) = (uint16_t)word;
-                    if (u % (GS / 4) == 0u)
-                        *reinterpret_cast<uint32_t*>(cell + (side ? kv4_value_step(D, GS, at.r, u / (GS / 4)) : kv4_key_step(D, GS, at.r, u / (GS / 4)))) =
-                            pack2<DT>(step, lo);
+            for (int o = 1; o < GL; o *= 2) range = min2<DT>(range, __shfl_xor_sync(0xffffffffu, range, o));
+            const float2 lh = unpack2<DT>(range);
+            float lo = lh.x, step = step_of<DT>(lo, -lh.y);
+            if (no_number<DT>(range)) { lo = __int_as_float(0x7fc00000); step = 0.0f; }
+            const uint32_t word = code_word<DT>(raw, lo, step);
+            if (live) {
+                uint8_t* cell = at.cell + (size_t)h * c.page_bytes;
+                if (!side) {
+                    *reinterpret_cast<uint32_t*>(cell + kv4_key_word(D, at.r, e / 4u)) = word;       // its halves are neighbours
+                } else {
+                    *reinterpret_cast<uint16_t*>(cell + kv4_value_word(D, at.r, e / 4u)) = (uint16_t)word;
+                    *reinterpret_cast<uint16_t*>(cell + kv4_value_word(D, at.r, e / 4u + 1u)) = (uint16_t)(word >> 16);
                 }
+                if (e % GS == 0u)
+                    *reinterpret_cast<uint32_t*>(cell + (side ? kv4_value_step(D, GS, at.r, e / GS) : kv4_key_step(D, GS, at.r, e / GS))) = pack2<DT>(step, lo);
             }
         }
     }
 }
 
 // ---- rows out of the cache -----------------------------------------------------------------------------------
-// the smaller, NaN if one is
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 // Bound by memory.  Warps and lanes as in append.
 template <int DT, int D, int GS>
 __global__ void __launch_bounds__(256) gather_kernel(Kv4Cache c, const void* slots, int wide, void* k_out, void* v_out, uint32_t tokens, uint32_t chunks,
                                                      uint32_t rounds, unsigned* err) {
     using T = typename Tr<DT>::T;
-    constexpr uint32_t BL = D < 128 ? D : 128, LANES = BL / 4, UNITS = D / BL, PER_WARP = 32 / LANES;
-    const float most = DT == FP16 ? 65504.0f : 3.38953139e38f;
+    using L = Lanes<D>;
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31u, all = c.kv_heads * UNITS;
+    const uint32_t lane = threadIdx.x & 31u, all = c.kv_heads * L::kUnits;
+    const bool side = lane >= 16u;
     const uint64_t items = (uint64_t)tokens * chunks;
     for (uint64_t i = (uint64_t)blockIdx.x * (blockDim.x / 32u) + (threadIdx.x >> 5); i < items; i += (uint64_t)gridDim.x * (blockDim.x / 32u)) {
         const uint32_t t = quotient(i, chunks), chunk = (uint32_t)(i - (uint64_t)t * chunks);
         const Place at = place_of(c, slots, wide, t, kv4_cell_bytes(D, GS), lane == 0u && chunk == 0u, err);
-        const uint32_t first = chunk * rounds * PER_WARP + lane / LANES;
-#pragma unroll 2
-        for (uint32_t round = 0; round < rounds; ++round) {
-            const uint32_t unit = first + round * PER_WARP;
-            if (unit >= all) break;
-            const uint32_t h = unit / UNITS, u = unit % UNITS * (BL / 4) + lane % LANES, g = u / (GS / 4);
-            const uint8_t* cell = at.cell + (size_t)h * c.page_bytes;
-            uint32_t w[2] = {0, 0}, s[2] = {0, 0};
-            if (at.inside) {
-                w[0] = *reinterpret_cast<const uint16_t*>(cell + kv4_key_word(D, at.r, u));
-                w[1] = *reinterpret_cast<const uint16_t*>(cell + kv4_value_word(D, at.r, u));
-                s[0] = *reinterpret_cast<const uint32_t*>(cell + kv4_key_step(D, GS, at.r, g));
-                s[1] = *reinterpret_cast<const uint32_t*>(cell + kv4_value_step(D, GS, at.r, g));
-            }
+        const uint32_t first = chunk * rounds * L::kRound + (lane & 15u) / L::kUnit;
+        T* row = reinterpret_cast<T*>(side ? v_out : k_out) + (size_t)t * c.kv_heads * D;
+        uint32_t all_w[kRounds], all_s[kRounds];
 #pragma unroll
-            for (int side = 0; side < 2; ++side) {
-                const float2 st = unpack2<DT>(s[side]);
-                float f[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)                              // 2^23 + code, less 2^23; a rounded step may lead beyond the type
-                    f[j] = min_nan(fmaf(__uint_as_float((w[side] >> (4 * j) & 15u) | 0x4b000000u) - 8388608.0f, st.x, st.y), most);
-                T* dst = reinterpret_cast<T*>(side ? v_out : k_out) + ((size_t)t * c.kv_heads + h) * D + 4u * u;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]));
+        for (uint32_t round = 0; round < kRounds; ++round) {         // everything that the warp reads is under way at once
+            const uint32_t unit = first + round * L::kRound, h = unit / L::kUnits, e = unit % L::kUnits * L::kBlock + lane % L::kUnit * 8u;
+            all_w[round] = all_s[round] = 0u;
+            if (at.inside && round < rounds && unit < all) {
+                const uint8_t* cell = at.cell + (size_t)h * c.page_bytes;
+                all_w[round] = side ? (uint32_t)*reinterpret_cast<const uint16_t*>(cell + kv4_value_word(D, at.r, e / 4u)) |
+                                          (uint32_t)*reinterpret_cast<const uint16_t*>(cell + kv4_value_word(D, at.r, e / 4u + 1u)) << 16
+                                    : *reinterpret_cast<const uint32_t*>(cell + kv4_key_word(D, at.r, e / 4u));
+                all_s[round] = *reinterpret_cast<const uint32_t*>(cell + (side ? kv4_value_step(D, GS, at.r, e / GS) : kv4_key_step(D, GS, at.r, e / GS)));
             }
+        }
+#pragma unroll
+        for (uint32_t round = 0; round < kRounds; ++round) {
+            if (round >= rounds) break;
+            const uint32_t unit = first + round * L::kRound, h = unit / L::kUnits, e = unit % L::kUnits * L::kBlock + lane % L::kUnit * 8u;
+            const uint32_t w = all_w[round], s = all_s[round];
+            // offset + step * code in one rounding, kept finite (a rounded step may lead beyond the type): pairs (0, 4), (1, 5), (2, 6), (3, 7)
+            constexpr uint32_t BASE = DT == FP16 ? 0x64006400u : 0x43004300u, MOST = DT == FP16 ? 0x7bff7bffu : 0x7f7f7f7fu;      // 1024 or 128
+            const auto step2 = as2<DT>(__byte_perm(s, 0, 0x1010)), lo2 = as2<DT>(__byte_perm(s, 0, 0x3232));
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                o[j] = min2<DT>(bits2<DT>(__hfma2(__hsub2(as2<DT>((w >> (4 * j) & 0x000f000fu) | BASE), as2<DT>(BASE)), step2, lo2)), MOST);
+            if (unit < all)
+                *reinterpret_cast<uint4*>(row + (size_t)h * D + e) = make_uint4(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410),
+                                                                               __byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
         }
     }
 }
 
-// how a token's heads are cut: one warp takes them all while there are tokens enough to fill the device, else fewer
+// how a token's heads are cut: up to four rounds to a warp while there are tokens enough to fill the device, else fewer
 struct Cut {
     uint32_t chunks, rounds, blocks;
 };
 Cut cut_heads(uint32_t tokens, uint32_t kv_heads, uint32_t d) {
-    const uint32_t widths = (kv_heads * d + 127u) / 128u;                  // warps' widths of a token
-    const uint32_t want = device_sms() * 96u;                              // warps, three times what an SM holds
+    const uint32_t widths = (kv_heads * d + 127u) / 128u;                  // rounds of a token
+    const uint32_t want = device_sms() * 32u;                              // warps
     Cut c;
     c.chunks = tokens >= want ? 1u : (want + tokens - 1u) / tokens;
+    if (c.chunks < (widths + kRounds - 1u) / kRounds) c.chunks = (widths + kRounds - 1u) / kRounds;
     if (c.chunks > widths) c.chunks = widths;
     c.rounds = (widths + c.chunks - 1u) / c.chunks;
     c.chunks = (widths + c.rounds - 1u) / c.rounds;
-    const uint64_t blocks = ((uint64_t)tokens * c.chunks + 7u) / 8u, most = (uint64_t)device_sms() * 8u;
-    c.blocks = (uint32_t)(blocks < most ? blocks : most);
+    const uint64_t blocks = ((uint64_t)tokens * c.chunks + 7u) / 8u;
+    c.blocks = (uint32_t)(blocks < 0x40000000ull ? blocks : 0x40000000ull);
     return c;
 }
 
@@ -604,7 +625,7 @@ int decdec_kv4_append(const void* k, int64_t k_token, int64_t k_head, const void
     if (int r = stream_error_word(s, &err)) return r;
     const Kv4Cache c = make_cache(cache, pages, page_size, kv_heads, head_dim, group_size);
     const Rows rk{k, k_token, k_head}, rv{v, v_token, v_head};
-    const bool vec = aligned(k, k_token, k_head, 4, 2) && aligned(v, v_token, v_head, 4, 2);
+    const bool vec = aligned(k, k_token, k_head, 8, 2) && aligned(v, v_token, v_head, 8, 2);
     return launched(for_format(dtype, head_dim, group_size, AppendCall{rk, rv, slots, slots_wide, c, tokens, vec, err, s}), "append launch");
 }
 
@@ -613,7 +634,7 @@ int decdec_kv4_gather(const void* cache, uint32_t pages, uint32_t page_size, uin
     if (int r = check_format(dtype, head_dim, group_size, page_size, cache, pages, kv_heads)) return r;
     if (tokens == 0) return 0;
     if (!k_out || !v_out || !slots) return fail(DECDEC_E_INVALID, "null pointer argument");
-    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 7u) return fail(DECDEC_E_INVALID, "outputs must be 8-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u) return fail(DECDEC_E_INVALID, "outputs must be 16-byte aligned");
     if ((uint64_t)tokens * kv_heads > 0x7fffffffull) return fail(DECDEC_E_UNSUPPORTED, "too many rows");
     unsigned* err = nullptr;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -121,14 +121,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> plan(const Tensor& le
     TORCH_CHECK(tokens >= 0 && tokens <= kMost, "tokens must be from 0 to 2^31 - 1.");
     TORCH_CHECK(page_size > 0 && page_size <= kMost, "page_size must be a multiple of 16 up to 65536, got ", page_size);
     c10::cuda::CUDAGuard guard(lengths.device());
-    const Tensor positions = at::empty({tokens}, lengths.options().dtype(at::kLong)), slots = at::empty({tokens}, positions.options());
-    const Tensor small = at::empty({2 * requests + 3}, lengths.options());
-    const Tensor starts = small.narrow(0, 0, requests + 1), after = small.narrow(0, requests + 1, requests), left = small.narrow(0, 2 * requests + 1, 1),
-                 status = small.narrow(0, 2 * requests + 2, 1);
-    int32_t* s = small.data_ptr<int32_t>();
+    // an allocation is cheaper than a view
+    const auto wide = lengths.options().dtype(at::kLong);
+    const Tensor positions = at::empty({tokens}, wide), slots = at::empty({tokens}, wide), starts = at::empty({requests + 1}, lengths.options()),
+                 after = at::empty({requests}, lengths.options()), left = at::empty({1}, lengths.options()), status = at::empty({1}, lengths.options());
     ok(decdec_kv4_plan(len, add, (uint32_t)requests, block_table.data_ptr<int32_t>(), block_table.stride(0), (uint32_t)block_table.size(1), pages,
-                       (uint32_t)free_pages.numel(), count, (uint32_t)page_size, (uint32_t)tokens, positions.data_ptr<int64_t>(), slots.data_ptr<int64_t>(), s,
-                       s + requests + 1, s + 2 * requests + 1, s + 2 * requests + 2, stream_of(lengths)));
+                       (uint32_t)free_pages.numel(), count, (uint32_t)page_size, (uint32_t)tokens, positions.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
+                       starts.data_ptr<int32_t>(), after.data_ptr<int32_t>(), left.data_ptr<int32_t>(), status.data_ptr<int32_t>(), stream_of(lengths)));
     return {positions, slots, starts, after, left, status};
 }
 
