@@ -10,7 +10,7 @@
 // codes of one sign make sums that grow with the context and are cut off in one direction at every step.)  Tokens are the 16 rows of
 // an operand in the scores (m16n8k16, 8 queries wide) and its depth in the outputs, so a batch-1 token with 4 queries per key head
 // fills half of each instruction instead of a quarter.
-//   queries     fp16 after scaling each row to a power of two near 2^13: exact for both 16-bit types (elements below 2^-27 of the row's
+//   queries     fp16 after scaling each row to a power of two near 2^9: exact for both 16-bit types (elements below 2^-23 of the row's
 //               largest lose bits)
 //   weights     p_t * step_t in fp16 with the steps scaled by a running power of two per group, so that neither small steps nor
 //               small weights become subnormal before they are 2^-23 of the largest
@@ -59,6 +59,17 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }     // -126 <= e <= 127
+
+// the larger of each 16-bit pair, the number where one is NaN
+template <int DT> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    if constexpr (DT == FP16) {
+        const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
 
 // the codes of a word less 8, as fp16 pairs: (0, 4), (1, 5), (2, 6), (3, 7)
 __device__ __forceinline__ void code_pairs(uint32_t x, uint32_t (&h)[4]) {
@@ -311,8 +322,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
                 int e = (int)(__float_as_uint(most) >> 23) - 127;      // the row's exponent
-                e = (most > 0.0f && most < INFINITY) ? max(e, -87) : 13;
-                const float up = pow2(13 - e);
+                e = (most > 0.0f && most < INFINITY) ? max(e, -87) : 9;
+                const float up = pow2(9 - e);                          // and the raised codes bring 2^4
                 float sum[NG];
 #pragma unroll
                 for (int g = 0; g < NG; ++g) sum[g] = 0.0f;
@@ -330,8 +341,9 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 for (int g = 0; g < NG; ++g) {
                     sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
                     sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+                    sum[g] *= 16.0f;
                 }
-                const float mine_sf = p.scale_log2 * pow2(e - 13);
+                const float mine_sf = p.scale_log2 * pow2(e - 13);             // the sums with codes are 16 times too large
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     sf[nt][i] = __shfl_sync(0xffffffffu, mine_sf, 8 * tig + 4 * i);
@@ -391,14 +403,6 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                         load_words(kr[i], cell + kv4_key_step(D, GS, gid + 8 * i, 0));
                         load_words(vr[u][i], cell + kv4_value_step(D, GS, gid + 8 * i, 0));
                     }
-                    if (!clear) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            if (tok0 + 16 * u + 8 * i + gid >= rq.length) {            // behind the end lies what the page held before
-#pragma unroll
-                                for (int g = 0; g < NG; ++g) kr[i][g] = vr[u][i][g] = 0u;
-                            }
-                    }
                     uint32_t xa[NW / PER][PER], xb[NW / PER][PER];
 #pragma unroll
                     for (int bl = 0; bl < NW / PER; ++bl) {
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const float2 f = unpack2<DT>(kr[i][g]);
-                            ks[i] = 0.0625f * f.x;
+                            ks[i] = f.x;
                             ko[i] = fmaf(-64.0f, f.x, f.y);            // offset less the 1024 / 16 steps that the codes are raised by
                         }
 #pragma unroll
@@ -439,12 +443,6 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                             }
                     }
                 }
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[u][nt][i] *= sf[nt][i & 1];
                 bool poison = false;                          // a token that some row does not see holds no number: its product with 0 counts
                 if (!clear) {
 #pragma unroll
@@ -459,21 +457,27 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
-                            for (int g = 0; g < NG; ++g) poison |= !(fabsf(unpack2<DT>(vr[u][i][g]).y) < INFINITY);
+                            for (int g = 0; g < NG; ++g) {
+                                if (tok0 + 16 * u + 8 * i + gid >= rq.length) vr[u][i][g] = 0u;      // behind the end lies what the page held before
+                                poison |= !(fabsf(unpack2<DT>(vr[u][i][g]).y) < INFINITY);
+                            }
                     }
                     poison = __any_sync(0xffffffffu, poison);
                 }
+                // the step's largest scores and steps of the values
+                float high[NT][2], steps[NG];
                 bool follow = false;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        follow |= fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i])) > m[nt][i] + kGrow;
-                }
+                    for (int i = 0; i < 2; ++i) {
+                        high[nt][i] = fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i])) * sf[nt][i];
+                        follow |= high[nt][i] > m[nt][i] + kGrow;
+                    }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const float top = fmaxf(fmaxf(unpack2<DT>(vr[0][0][g]).x, unpack2<DT>(vr[0][1][g]).x), fmaxf(unpack2<DT>(vr[1][0][g]).x, unpack2<DT>(vr[1][1][g]).x));
-                    follow |= top > limit[g];
+                    steps[g] = unpack2<DT>(max2<DT>(max2<DT>(vr[0][0][g], vr[0][1][g]), max2<DT>(vr[1][0][g], vr[1][1][g]))).x;
+                    follow |= steps[g] > limit[g];
                 }
                 if (__any_sync(0xffffffffu, follow)) {
                     // maxima over the step, sums brought to them; rare once a few cells are done
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float top = fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i]));
+                            float top = high[nt][i];
 #pragma unroll
                             for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             top = fmaxf(top, m[nt][i]);
@@ -493,8 +497,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                         }
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
-                        const float top = fmaxf(fmaxf(unpack2<DT>(vr[0][0][g]).x, unpack2<DT>(vr[0][1][g]).x), fmaxf(unpack2<DT>(vr[1][0][g]).x, unpack2<DT>(vr[1][1][g]).x));
-                        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(top, 0.0f)));
+                        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(steps[g], 0.0f)));
                         const int e = min(max((int)(bits >> 23) - 127, -100), 100);   // the largest step is below 2^(e+1)
                         const float want = pow2(10 - e);
                         float by = 1.0f;
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            w[nt][i] = ex2(s[u][nt][i] - less[nt][i & 1]);
+                            w[nt][i] = ex2(fmaf(s[u][nt][i], sf[nt][i & 1], -less[nt][i & 1]));
                             l[nt][i & 1] += w[nt][i];
                         }
                     // ---- outputs: rows = elements, depth = tokens, columns = queries; planes of tokens 0..7 and 8..15
