@@ -82,7 +82,7 @@ int decdec_kv4_attention(const void* q, int64_t q_token, int64_t q_head, void* o
         return fail(DECDEC_E_INVALID, "page_size must be a multiple of 16 up to 65536, got %llu", page_size);
     if (pages == 0 || pages > 0x7fffffffu) return fail(DECDEC_E_INVALID, "empty cache or too many pages");
     if ((uint64_t)pages * kv_heads * (page_size / kCellTokens) >= kNoCell) return fail(DECDEC_E_UNSUPPORTED, "the cache has more cells than 32 bits count");
-    if ((uint64_t)table_cols * page_size > 0x7fffffffull) return fail(DECDEC_E_INVALID, "the tokens of a table row must stay below 2^31");
+    if ((uint64_t)table_cols * page_size > 0x7ffffe00ull) return fail(DECDEC_E_INVALID, "the tokens of a table row must stay below 2^31 - 512");
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(DECDEC_E_INVALID, "scale must be a positive number");
     if (rows == 0) return 0;
     if (!q || !out || !cache || (requests && (!lengths || !query_starts)) || (requests && table_cols && !table)) return fail(DECDEC_E_INVALID, "null pointer argument");

@@ -152,9 +152,9 @@ template <int D, int NT> struct DecodeShape {
 };
 // A step of a warp is two neighbouring cells (32 tokens), and kStages steps of a warp lie in shared memory, beside the place where the
 // warps' sums are added: the next segment's first steps are under way meanwhile.
-constexpr int kStages = 3;
+constexpr int kStages = 3, kCells = 2;
 template <int D, int GS, int NT> __host__ __device__ constexpr size_t decode_smem() {
-    return (size_t)kDecodeWarps * kStages * 2u * kv4_cell_bytes(D, GS) + DecodeShape<D, NT>::kMergeFloats * 4u;
+    return (size_t)kDecodeWarps * kStages * (uint32_t)kCells * kv4_cell_bytes(D, GS) + DecodeShape<D, NT>::kMergeFloats * 4u;
 }
 
 // blocks of an SM that the registers are cut for: as many as need no spills worth the name
@@ -176,9 +176,9 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gid = lane >> 2, tig = lane & 3;
-    uint8_t* ring = smem + (size_t)warp * kStages * 2 * CELL;
+    uint8_t* ring = smem + (size_t)warp * kStages * kCells * CELL;
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-    float* merge = reinterpret_cast<float*>(smem + (size_t)kDecodeWarps * kStages * 2 * CELL);   // [warp][row][kRowStride]
+    float* merge = reinterpret_cast<float*>(smem + (size_t)kDecodeWarps * kStages * kCells * CELL);   // [warp][row][kRowStride]
     float* merge_ml = merge + kDecodeWarps * Sh::kRows * Sh::kRowStride;                      // [warp][row][2]
     uint8_t* after = reinterpret_cast<uint8_t*>(p.part + (size_t)gridDim.x * 2u * kv4_part_floats(D, NT));
     Kv4Cut* cuts = reinterpret_cast<Kv4Cut*>(after);
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
         int count;
         uint32_t cell_at, fill;                              // place in the cache of the cell 2 j + lane of its steps; stage that is filled next
         auto places_of = [&](int j0) {
-            const int c = rq.first + c0 + 2 * (warp + kDecodeWarps * (j0 + (lane >> 1))) + (lane & 1);
+            const int c = rq.first + c0 + kCells * (warp + kDecodeWarps * (j0 + lane / kCells)) + lane % kCells;
             cell_at = kNoCell;
             if (c < rq.first + c1 && c * kCellTokens < rq.length) {
                 const uint32_t column = (uint32_t)c / p.page_cells;
@@ -258,22 +258,22 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
         };
         auto issue = [&](int j) {
             if (j < count) {
-                if ((j & 15) == 0) places_of(j);
+                if (j % (32 / kCells) == 0) places_of(j);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t at = __shfl_sync(0xffffffffu, cell_at, 2 * (j & 15) + u);
+                for (int u = 0; u < kCells; ++u) {
+                    const uint32_t at = __shfl_sync(0xffffffffu, cell_at, kCells * (j % (32 / kCells)) + u);
                     const uint32_t bytes = at == kNoCell ? 0u : 16u;       // zeros, from a source that is not read
                     const uint8_t* src = p.cache + (size_t)(at == kNoCell ? 0u : at) * CELL + lane * 16u;
 #pragma unroll
                     for (uint32_t i = 0; i < (CELL / 16 + 31) / 32; ++i)
                         if (CELL % 512 == 0 || i * 512u + lane * 16u < CELL) cp_async16(fill + u * CELL + i * 512u, src + i * 512u, bytes);
                 }
-                fill = fill == ring_s + lane * 16u + (kStages - 1) * 2u * CELL ? ring_s + lane * 16u : fill + 2u * CELL;
+                fill = fill == ring_s + lane * 16u + (kStages - 1u) * kCells * CELL ? ring_s + lane * 16u : fill + kCells * CELL;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         auto begin = [&] {
-            count = ((c1 - c0 + 1) / 2 - warp + kDecodeWarps - 1) / kDecodeWarps;
+            count = ((c1 - c0 + kCells - 1) / kCells - warp + kDecodeWarps - 1) / kDecodeWarps;
             fill = ring_s + lane * 16u;
 #pragma unroll
             for (int j = 0; j < kStages - 1; ++j) issue(j);
@@ -392,10 +392,10 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 constexpr int PER = NW < 4 ? NW : 4;          // words of a lane in a block
                 constexpr int VB = D < 128 ? 1 : D / 128, VP = NW / VB;      // blocks of values, words of a lane and plane in each
                 // ---- scores: rows = tokens gid, gid + 8 of cell u; columns = queries 2 tig, 2 tig + 1
-                float s[2][NT][4];
-                uint32_t vr[2][2][NG];                        // steps and offsets of the values
+                float s[kCells][NT][4];
+                uint32_t vr[kCells][2][NG];                        // steps and offsets of the values
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < kCells; ++u) {
                     const uint8_t* cell = st + u * CELL;
                     uint32_t kr[2][NG];
 #pragma unroll
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 bool poison = false;                          // a token that some row does not see holds no number: its product with 0 counts
                 if (!clear) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                    for (int u = 0; u < kCells; ++u) {
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -471,12 +471,18 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        high[nt][i] = fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i])) * sf[nt][i];
+                        float top = fmaxf(s[0][nt][i], s[0][nt][2 + i]);
+#pragma unroll
+                        for (int u = 1; u < kCells; ++u) top = fmaxf(top, fmaxf(s[u][nt][i], s[u][nt][2 + i]));
+                        high[nt][i] = top * sf[nt][i];
                         follow |= high[nt][i] > m[nt][i] + kGrow;
                     }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    steps[g] = unpack2<DT>(max2<DT>(max2<DT>(vr[0][0][g], vr[0][1][g]), max2<DT>(vr[1][0][g], vr[1][1][g]))).x;
+                    uint32_t top = max2<DT>(vr[0][0][g], vr[0][1][g]);
+#pragma unroll
+                    for (int u = 1; u < kCells; ++u) top = max2<DT>(top, max2<DT>(vr[u][0][g], vr[u][1][g]));
+                    steps[g] = unpack2<DT>(top).x;
                     follow |= steps[g] > limit[g];
                 }
                 if (__any_sync(0xffffffffu, follow)) {
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < kCells; ++u) {
                     const uint8_t* cell = st + u * CELL;
                     float w[NT][4];
 #pragma unroll
@@ -570,15 +576,15 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                 }
             };
             const uint8_t* st = ring;
-            int tok0 = (rq.first + c0 + 2 * warp) * kCellTokens;
+            int tok0 = (rq.first + c0 + kCells * warp) * kCellTokens;
             for (int j = 0; j < count; ++j) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
                 __syncwarp();
                 issue(j + kStages - 1);                      // into the stage that the last step read
                 // behind the end of the segment's cells lies another block's work: `to` hides it
-                step(st, tok0, tok0 >= clear_from && tok0 + 2 * kCellTokens <= clear_to);
-                st = st == ring + (kStages - 1) * 2 * CELL ? ring : st + 2 * CELL;
-                tok0 += kDecodeWarps * 2 * kCellTokens;
+                step(st, tok0, tok0 >= clear_from && tok0 + kCells * kCellTokens <= clear_to);
+                st = st == ring + (kStages - 1) * kCells * CELL ? ring : st + kCells * CELL;
+                tok0 += kDecodeWarps * kCells * kCellTokens;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();                                    // the warp is through with its ring

@@ -35,6 +35,31 @@ void on_gpu(const Tensor& first, std::initializer_list<const Tensor*> others) {
     for (const Tensor* t : others) TORCH_CHECK(!t || t->device() == first.device(), "all tensors must be on the same GPU.");
 }
 
+constexpr const char* kOverlap = "an output must not share memory with itself, another output or an input.";
+
+// rows [tokens][heads][d]: elements from the first to the last of a token
+int64_t extent(const Tensor& t) { return (t.size(1) - 1) * t.stride(1) + t.size(2); }
+bool same(const Tensor& a, const Tensor& b) { return a.data_ptr() == b.data_ptr() && a.strides() == b.strides(); }
+// whether no two elements of t share a place (views whose heads or tokens are wound into one another count as sharing)
+bool spread(const Tensor& t) {
+    return t.numel() == 0 || ((t.size(1) == 1 || t.stride(1) >= t.size(2)) && (t.size(0) == 1 || t.stride(0) >= extent(t)));
+}
+// whether a and b share no place: ranges apart, or the same token stride and different parts of it (parts of a fused projection), or the
+// same head stride and different parts of that.  What it cannot tell counts as sharing.
+bool apart(const Tensor& a, const Tensor& b) {
+    if (!a.numel() || !b.numel()) return true;
+    const int64_t size = a.element_size(), pa = (int64_t)a.data_ptr() / size, pb = (int64_t)b.data_ptr() / size;
+    const int64_t ea = extent(a), eb = extent(b), la = (a.size(0) - 1) * a.stride(0) + ea, lb = (b.size(0) - 1) * b.stride(0) + eb;
+    if (pa + la <= pb || pb + lb <= pa) return true;
+    auto within = [&](int64_t period, int64_t na, int64_t nb) {
+        if (period <= 0) return false;
+        const int64_t d = ((pb - pa) % period + period) % period;
+        return d >= na && d + nb <= period;
+    };
+    if (a.stride(0) == b.stride(0) && within(a.stride(0), ea, eb)) return true;
+    return a.stride(1) == b.stride(1) && a.stride(0) == b.stride(0) && a.stride(1) > 0 && a.stride(0) % a.stride(1) == 0 && within(a.stride(1), a.size(2), b.size(2));
+}
+
 const Tensor* at_or_null(const Maybe& t) { return t ? &*t : nullptr; }
 
 int index(const Tensor& t, int64_t n, const char* name) {
@@ -96,6 +121,12 @@ std::tuple<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& 
         TORCH_CHECK(!k || (k_out->sizes() == k->sizes() && k_out->scalar_type() == k->scalar_type()), "out must have the shapes and types of q and k.");
         rows(*q_out, "out");
         if (k_out) rows(*k_out, "out");
+        // an output may be its own input, and shares memory with nothing else that is read or written
+        TORCH_CHECK(spread(*q_out) && (same(*q_out, q) || apart(*q_out, q)), kOverlap);
+        if (k) {
+            TORCH_CHECK(spread(*k_out) && (same(*k_out, *k) || apart(*k_out, *k)), kOverlap);
+            TORCH_CHECK(apart(*q_out, *k) && apart(*k_out, q) && apart(*k_out, *q_out), kOverlap);
+        }
         qo = *q_out;
         ko = k_out;
     } else {
@@ -116,6 +147,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> plan(const Tensor& le
     const int32_t* len = int32s(lengths, -1, "lengths");
     const int32_t* add = int32s(fresh, requests, "new_lengths");
     table(block_table, requests);
+    TORCH_CHECK(requests <= 1 || block_table.stride(0) >= block_table.size(1), "rows of block_table must not overlap, it is written.");
     const int32_t* pages = int32s(free_pages, -1, "free_pages");
     const int32_t* count = int32s(free_count, 1, "free_count");
     TORCH_CHECK(tokens >= 0 && tokens <= kMost, "tokens must be from 0 to 2^31 - 1.");
@@ -179,6 +211,7 @@ std::tuple<Tensor, Maybe> attention(const Tensor& q, const Tensor& cache, const 
     if (out_given) {
         TORCH_CHECK(out_given->sizes() == q.sizes() && out_given->scalar_type() == q.scalar_type(), "out must have the shape and type of q.");
         rows(*out_given, "out");
+        TORCH_CHECK(spread(*out_given) && apart(*out_given, q), kOverlap);
         out = *out_given;
     } else {
         out = at::empty({tokens, heads, d}, q.options());

@@ -5,6 +5,8 @@ import numpy as np
 import torch
 
 HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}     # half a step, relative
+# and half a step of the subnormal numbers: fp16 outputs below 2^-14 lie 2^-24 apart, whatever their size
+SUBNORMAL = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}
 
 
 def quantize(x, group):
@@ -125,7 +127,7 @@ def attention(q, k, v, length, scale, window, group, dense=False):
         worst = torch.where(seen, mag, 0.0).nan_to_num(0.0).amax(-1, keepdim=True)
         a, w = p @ away[:, g].nan_to_num(0.0), p @ whole[:, g].nan_to_num(0.0)
         bound[:, h] = HALF[q.dtype] * (out[:, h].abs() + w * 2.0 ** -9) + 2.0 ** -11 * a + (2.0 ** -10 * 2.0 ** -4 + 2.0 ** -19 * worst) * w + \
-            length * 2.0 ** -28 * whole[:, g].nan_to_num(0.0).amax(0) + 1e-30
+            length * 2.0 ** -28 * whole[:, g].nan_to_num(0.0).amax(0) + SUBNORMAL[q.dtype]
         if dense:
             middle = klo + 8 * kstep
             size = kd.abs() + middle.abs().repeat_interleave(group, -1)

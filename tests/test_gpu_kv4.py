@@ -360,9 +360,10 @@ def test_attention_poison_behind_the_mask(kv4, queries):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("kind", ["uniform", "sharp", "rising", "large", "tiny"])
-def test_attention_of_extreme_scores_and_values(kv4, dtype, kind):
-    b = Batch(kv4, [500, 33], [1, 2], 8, 2, 128, 32, dtype, 32, 500)
+@pytest.mark.parametrize("kind", ["uniform", "sharp", "rising", "large", "tiny", "silent"])
+@pytest.mark.parametrize("queries", [2, 33])
+def test_attention_of_extreme_scores_and_values(kv4, dtype, kind, queries):
+    b = Batch(kv4, [500, 33], [1, queries], 8, 2, 128, 32, dtype, 32, 500)
     if kind == "uniform":
         b.q.zero_()
     elif kind == "sharp":
@@ -377,6 +378,10 @@ def test_attention_of_extreme_scores_and_values(kv4, dtype, kind):
         for k, v in zip(b.k, b.v):
             k *= 0.01
             v *= 5000
+    elif kind == "silent":                                             # no values at all for the first tokens, then some
+        for k, v in zip(b.k, b.v):
+            v[:20] = 0
+            v[20:] *= 3
     else:
         for k, v in zip(b.k, b.v):
             v *= 2.0 ** -9
@@ -398,6 +403,70 @@ def test_attention_does_not_depend_on_how_the_work_is_cut(kv4):
         alone = kv4.attention(b.q[i:i + 1].cuda(), b.cache, b.table[i:i + 1].cuda(), torch.tensor([lengths[i]], dtype=torch.int32).cuda(),
                               torch.tensor([0, 1], dtype=torch.int32).cuda(), 128)
         assert (alone[0].double() - out[i].double()).abs().max() <= 2.0 ** -10 * out[i].abs().max() + 2e-4
+
+
+@pytest.mark.parametrize("queries", [1, 40])
+def test_attention_near_the_ends_of_bf16(kv4, queries):
+    """Queries, keys and values of magnitudes that fp16 does not hold: scaled to it by powers of two, here and there with zeros."""
+    b = Batch(kv4, [300, 64], [queries, 1], 8, 2, 128, 64, torch.bfloat16, 16, 650)
+    b.q *= 2.0 ** 90
+    for k, v in zip(b.k, b.v):
+        k *= 2.0 ** -90
+        v *= 2.0 ** 100
+        v[3::7] = 0
+    b.fill()
+    out, lse = b.run(return_lse=True)
+    b.check(out, lse)
+    for k, v in zip(b.k, b.v):
+        k *= 2.0 ** 60
+        v *= 2.0 ** -190
+    b.q *= 2.0 ** -60
+    b.fill()
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("most", [1, 3, 500])
+def test_attention_with_any_bound_of_queries(kv4, most):
+    """max_queries chooses the kernel; requests with more rows, and with fewer, are computed all the same."""
+    b = Batch(kv4, [150, 3, 64], [77, 1, 20], 8, 2, 128, 128, torch.bfloat16, 16, 660)
+    out = b.run(max_queries=most)
+    b.check(out)
+
+
+def test_attention_without_requests_or_pages(kv4):
+    q = normal((5, 4, 64), torch.float16, 41).cuda()
+    cache = kv4.empty_cache(2, 16, 2, 64, 64)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out, lse = kv4.attention(q, cache, none.view(0, 3), none, torch.zeros(1, dtype=torch.int32, device="cuda"), 64, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    starts = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda")
+    out = kv4.attention(q, cache, none.view(2, 0), torch.zeros(2, dtype=torch.int32, device="cuda"), starts, 64)
+    assert (out == 0).all()
+
+
+def test_overlapping_outputs_are_refused(kv4):
+    frequencies, _ = kv4.rotary_frequencies(64)
+    x = normal((4, 4, 64), torch.float16, 42).cuda()
+    pos = torch.zeros(4, dtype=torch.int64, device="cuda")
+    with pytest.raises(RuntimeError):
+        kv4.rotary(x[:, :2], x[:, 2:], pos, frequencies, out=(x[:, :2], x[:, :2]))
+    with pytest.raises(RuntimeError):
+        kv4.rotary(x, None, pos, frequencies, out=(x[:1].expand(4, 4, 64), None))
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        kv4.rotary(x[:3], None, pos[:3], frequencies, out=(x[1:], None))          # the same rows shifted by one
+    packed = normal((4, 3, 3, 64), torch.float16, 43).cuda()                      # queries, keys and values side by side in every head
+    q, k = packed[:, :, 0], packed[:, :, 1]
+    want = kv4.rotary(q, k, pos + 5, frequencies)
+    keep = packed[:, :, 2].clone()
+    kv4.rotary(q, k, pos + 5, frequencies, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(packed[:, :, 2], keep)
+    b = Batch(kv4, [9], [4], 4, 2, 64, 64, torch.float16, 16, 670)
+    with pytest.raises(RuntimeError):
+        kv4.attention(x, b.cache, b.table.cuda(), torch.tensor([9], dtype=torch.int32).cuda(), b.starts.cuda(), 64, out=x)
+    one = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    n = torch.ones(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        kv4.plan(n, n, one.expand(2, 4), n, n[:1], 16, 2)
 
 
 def test_attention_many_requests(kv4):
