@@ -119,8 +119,8 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm vol
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
 // Bounded: after about half a second the block gives up, here and in every later wait.
@@ -149,27 +149,6 @@ struct __align__(16) ChunkMeta {
     int key_exp[4], value_exp[4];
     uint32_t any_poison[4], poison[4][4];
 };
-
-__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 of_pair(unsigned long long v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 
 template <int D, int GS, int DT>
 __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) {
@@ -613,19 +592,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                             }
                         }
                         const float less = (float)shift - (m == -INFINITY ? 0.0f : m);
-                        const unsigned long long by = pair_of(f, f), off = pair_of(less, less);
-                        unsigned long long sum = 0ull;
+                        float sum[2] = {0.0f, 0.0f};
                         uint32_t w[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            float2 x = of_pair(fma_pair(pair_of(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), by, off));
-                            x.x = ex2(x.x);
-                            x.y = ex2(x.y);
-                            sum = add_pair(sum, pair_of(x.x, x.y));
-                            w[i] = half2_bits(x.x, x.y);
+                            const float x = ex2(fmaf(__uint_as_float(r[2 * i]), f, less)), y = ex2(fmaf(__uint_as_float(r[2 * i + 1]), f, less));
+                            sum[0] += x;
+                            sum[1] += y;
+                            w[i] = half2_bits(x, y);
                         }
-                        const float2 part = of_pair(sum);
-                        l = fmaf(part.x + part.y, pow2(-shift), l);
+                        l = fmaf(sum[0] + sum[1], pow2(-shift), l);
                         tmem_store16(at_s + 16 * c, w);
                     }
                     ev = new_ev;
