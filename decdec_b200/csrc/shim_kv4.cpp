@@ -2,6 +2,7 @@
 // libdecdec_b200.so.  It checks tensors, allocates outputs and the workspace of attention on the current stream, and turns status
 // codes into RuntimeError.  (Through ctypes the same calls cost 26 to 41 us of host time, more than most of the kernels.)
 #include <torch/extension.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/stl.h>
@@ -23,6 +24,16 @@ bool is16(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
 void ok(int code) { TORCH_CHECK(code == 0, decdec_last_error()); }
 void* stream_of(const Tensor& t) { return static_cast<void*>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()); }
+
+// memory of the caching allocator without the way through the dispatcher, which costs as much again
+Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) { return at::detail::empty_cuda(sizes, type, device, std::nullopt); }
+// n elements of a contiguous tensor from element `at` on: a view that only these functions hand out
+Tensor part(const Tensor& base, int64_t at, int64_t n) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(base.storage()), base.key_set(), base.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(base.storage_offset() + at);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return t;
+}
 
 void rows(const Tensor& t, const char* name) {
     TORCH_CHECK(t.dim() == 3, name, " must be of shape (tokens, heads, head_dim).");
@@ -130,8 +141,8 @@ std::tuple<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& 
         qo = *q_out;
         ko = k_out;
     } else {
-        qo = at::empty({tokens, q.size(1), d}, q.options());
-        if (k) ko = at::empty({tokens, k->size(1), d}, q.options());
+        qo = empty({tokens, q.size(1), d}, q.scalar_type(), q.device());
+        if (k) ko = empty({tokens, k->size(1), d}, q.scalar_type(), q.device());
     }
     ok(decdec_rotary(q.data_ptr(), q.stride(0), q.stride(1), (uint32_t)q.size(1), k ? k->data_ptr() : nullptr, k ? k->stride(0) : 0, k ? k->stride(1) : 0,
                      k ? (uint32_t)k->size(1) : 0, qo.data_ptr(), qo.stride(0), qo.stride(1), ko ? ko->data_ptr() : nullptr, ko ? ko->stride(0) : 0,
@@ -153,13 +164,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> plan(const Tensor& le
     TORCH_CHECK(tokens >= 0 && tokens <= kMost, "tokens must be from 0 to 2^31 - 1.");
     TORCH_CHECK(page_size > 0 && page_size <= kMost, "page_size must be a multiple of 16 up to 65536, got ", page_size);
     c10::cuda::CUDAGuard guard(lengths.device());
-    // an allocation is cheaper than a view
-    const auto wide = lengths.options().dtype(at::kLong);
-    const Tensor positions = at::empty({tokens}, wide), slots = at::empty({tokens}, wide), starts = at::empty({requests + 1}, lengths.options()),
-                 after = at::empty({requests}, lengths.options()), left = at::empty({1}, lengths.options()), status = at::empty({1}, lengths.options());
+    const Tensor wide = empty({2 * tokens}, at::kLong, lengths.device()), narrow = empty({2 * requests + 3}, at::kInt, lengths.device());
+    const Tensor positions = part(wide, 0, tokens), slots = part(wide, tokens, tokens), starts = part(narrow, 0, requests + 1),
+                 after = part(narrow, requests + 1, requests), left = part(narrow, 2 * requests + 1, 1), status = part(narrow, 2 * requests + 2, 1);
+    int64_t* w = wide.data_ptr<int64_t>();
+    int32_t* n = narrow.data_ptr<int32_t>();
     ok(decdec_kv4_plan(len, add, (uint32_t)requests, block_table.data_ptr<int32_t>(), block_table.stride(0), (uint32_t)block_table.size(1), pages,
-                       (uint32_t)free_pages.numel(), count, (uint32_t)page_size, (uint32_t)tokens, positions.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
-                       starts.data_ptr<int32_t>(), after.data_ptr<int32_t>(), left.data_ptr<int32_t>(), status.data_ptr<int32_t>(), stream_of(lengths)));
+                       (uint32_t)free_pages.numel(), count, (uint32_t)page_size, (uint32_t)tokens, w, w + tokens, n,
+                       n + requests + 1, n + 2 * requests + 1, n + 2 * requests + 2, stream_of(lengths)));
     return {positions, slots, starts, after, left, status};
 }
 
@@ -185,7 +197,7 @@ std::tuple<Tensor, Tensor> gather(const Tensor& cache, const Tensor& slots, int6
     const int wide = index(slots, n, "slots");
     TORCH_CHECK(n <= kMost, "too many slots.");
     c10::cuda::CUDAGuard guard(cache.device());
-    const Tensor k = at::empty({n, c.kv_heads, head_dim}, cache.options().dtype(dtype)), v = at::empty({n, c.kv_heads, head_dim}, k.options());
+    const Tensor k = empty({n, c.kv_heads, head_dim}, dtype, cache.device()), v = empty({n, c.kv_heads, head_dim}, dtype, cache.device());
     ok(decdec_kv4_gather(c.p, c.pages, c.page_size, c.kv_heads, (uint32_t)head_dim, (uint32_t)group_size, slots.data_ptr(), wide, (uint32_t)n, k.data_ptr(),
                          v.data_ptr(), dt_of(dtype), stream_of(cache)));
     return {k, v};
@@ -214,14 +226,14 @@ std::tuple<Tensor, Maybe> attention(const Tensor& q, const Tensor& cache, const 
         TORCH_CHECK(spread(*out_given) && apart(*out_given, q), kOverlap);
         out = *out_given;
     } else {
-        out = at::empty({tokens, heads, d}, q.options());
+        out = empty({tokens, heads, d}, q.scalar_type(), q.device());
     }
     Maybe lse;
     if (return_lse) lse = at::full({tokens, heads}, -std::numeric_limits<double>::infinity(), q.options().dtype(at::kFloat));
     const int dt = dt_of(q.scalar_type());
     size_t bytes = 0;
     ok(decdec_kv4_attention_workspace((uint32_t)requests, (uint32_t)tokens, (uint32_t)heads, c.kv_heads, (uint32_t)d, (uint32_t)group_size, most, dt, &bytes));
-    const Tensor workspace = at::empty({(int64_t)bytes}, cache.options());
+    const Tensor workspace = empty({(int64_t)bytes}, at::kByte, q.device());
     ok(decdec_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse ? lse->data_ptr<float>() : nullptr, c.p,
                             c.pages, c.page_size, block_table.data_ptr<int32_t>(), block_table.stride(0), (uint32_t)block_table.size(1), len, starts,
                             (uint32_t)requests, (uint32_t)tokens, (uint32_t)heads, c.kv_heads, (uint32_t)d, (uint32_t)group_size, most,
