@@ -117,6 +117,7 @@ int decdec_kv4_attention(const void* q, int64_t q_token, int64_t q_head, void* o
         const uint64_t tiles = ((uint64_t)rows * ratio + 8u * c.nt - 1) / (8u * c.nt) + requests;
         const uint64_t cells = tiles * kv_heads * ((uint64_t)table_cols * p.page_cells + 1u);
         uint64_t blocks = (cells + 2 * kDecodeWarps - 1) / (2 * kDecodeWarps);
+        if (blocks < tiles * kv_heads) blocks = tiles * kv_heads;               // a block for every segment
         if (blocks > c.blocks) blocks = c.blocks;
         if (blocks == 0) blocks = 1;
         e = head_dim == 64    ? launch_kv4_decode64(group_size, c.nt, dtype, p, (uint32_t)blocks, s)

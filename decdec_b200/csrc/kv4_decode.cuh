@@ -17,7 +17,7 @@
 //   the rest    (scores, running maximum and sum, the middles' part, sums over thread blocks) in fp32
 //
 // The work is a line of cells (16 tokens of one key head), request by request, and every thread block takes an equal part of it
-// (lengths are on the device: each block sums them itself).  A warp streams its own cells through shared memory (cp.async, kStages
+// (lengths are on the device: each block sums them itself); work that would not fill the device is cut by segments instead.  A warp streams its own cells through shared memory (cp.async, kStages
 // cells ahead) and keeps its own running maximum and sums; the four warps of a block are added where a segment (one request, head and
 // tile of 8 or 16 query rows) ends.  A segment that blocks share leaves its parts in `part`, and kv4_join adds them.
 #pragma once
@@ -145,6 +145,11 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4Attn& p, uint32_t b, 
     return r;
 }
 
+// Pieces of a segment where each has a block to itself: one up to 16 cells (two steps of a warp; a step costs 0.8 us, a join 2), then of 8
+// cells.  One request with 8 key heads, this / blocks of 8 cells cut from the line (us): 16 tokens 6.9 / 31 (one block has all heads), 100 tokens
+// 7.3 / 11.4, 777 tokens 9.7 / 12.5, 3000 tokens 10.3 / 12.9.
+__host__ __device__ constexpr int kv4_pieces(int cells) { return cells <= 16 ? 1 : (cells + 7) / 8; }
+
 template <int D, int NT> struct DecodeShape {
     static constexpr int kRows = 8 * NT;
     static constexpr int kRowStride = D + 4;            // floats; keeps the warps' 16-byte stores apart by banks
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     constexpr int NW = D / 32;                  // words of 32 elements
     constexpr uint32_t CELL = kv4_cell_bytes(D, GS);
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_sum[kDecodeThreads / 32];
+    __shared__ long long s_sum[2][kDecodeThreads / 32];
     __shared__ long long s_rest;
     __shared__ uint32_t s_request;
 
@@ -186,43 +191,54 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     pdl_trigger();
     pdl_wait();
 
-    // ---- this block's part of the line of cells
+    // ---- this block's part of the line of cells; or, while there are blocks for every segment or piece of one, a segment or a piece
     const uint32_t run = (p.requests + kDecodeThreads - 1u) / kDecodeThreads;
     const uint32_t rb0 = min(tid * run, p.requests), rb1 = min(rb0 + run, p.requests);
-    long long mine = 0;
+    long long mine[2] = {0, 0};                                // cells, pieces
     for (uint32_t b = rb0; b < rb1; ++b) {
         const Kv4Request r = kv4_request(p, b, Sh::kRows, blockIdx.x == 0);
-        mine += (long long)r.tiles * p.kv_heads * r.cells;
+        mine[0] += (long long)r.tiles * p.kv_heads * r.cells;
+        mine[1] += (long long)r.tiles * p.kv_heads * kv4_pieces(r.cells);
     }
-    long long incl = mine;
+    long long incl[2] = {mine[0], mine[1]};
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const long long n = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += n;
-    }
-    if (lane == 31) s_sum[warp] = incl;
-    __syncthreads();
-    long long before = 0, total = 0;
+    for (int o = 1; o < 32; o *= 2)
 #pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) {
-        if (w < warp) before += s_sum[w];
-        total += s_sum[w];
-    }
-    // at least two cells a warp: a shorter part would spend its time in the joining of the parts
-    const long long per = max((long long)ratio_of(total + gridDim.x - 1, gridDim.x), 2ll * kDecodeWarps);
-    const long long x0 = (long long)blockIdx.x * per, x1 = min(x0 + per, total);
-    const long long excl = before + incl - mine;
-    if (x0 < x1 && excl <= x0 && x0 < excl + mine) {
-        long long at = excl;
-        uint32_t b = rb0;
-        for (;; ++b) {                                       // ends: x0 lies below the end of this run
-            const Kv4Request r = kv4_request(p, b, Sh::kRows, false);
-            const long long n = (long long)r.tiles * p.kv_heads * r.cells;
-            if (x0 < at + n) break;
-            at += n;
+        for (int i = 0; i < 2; ++i) {
+            const long long n = __shfl_up_sync(0xffffffffu, incl[i], o);
+            if (lane >= o) incl[i] += n;
         }
-        s_request = b;
-        s_rest = x0 - at;
+    if (lane == 31) { s_sum[0][warp] = incl[0]; s_sum[1][warp] = incl[1]; }
+    __syncthreads();
+    long long before[2] = {0, 0}, all[2] = {0, 0};
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (w < warp) before[i] += s_sum[i][w];
+            all[i] += s_sum[i][w];
+        }
+    const bool pieces = all[1] <= (long long)gridDim.x;
+    const int kind = pieces ? 1 : 0;
+    const long long total = pieces ? all[1] : all[0];
+    // at least two cells a warp: a shorter part would spend its time in the joining of the parts
+    const long long per = pieces ? 1 : max((long long)ratio_of(total + gridDim.x - 1, gridDim.x), 2ll * kDecodeWarps);
+    const long long at0 = (long long)blockIdx.x * per;
+    long long x0 = at0, x1 = min(at0 + per, total);
+    {
+        const long long excl = (pieces ? before[1] + incl[1] - mine[1] : before[0] + incl[0] - mine[0]), own = pieces ? mine[1] : mine[0];
+        if (x0 < x1 && excl <= x0 && x0 < excl + own) {
+            long long at = excl;
+            uint32_t b = rb0;
+            for (;; ++b) {                                   // ends: x0 lies below the end of this run
+                const Kv4Request r = kv4_request(p, b, Sh::kRows, false);
+                const long long n = (long long)r.tiles * p.kv_heads * (kind ? kv4_pieces(r.cells) : r.cells);
+                if (x0 < at + n) break;
+                at += n;
+            }
+            s_request = b;
+            s_rest = x0 - at;
+        }
     }
     __syncthreads();
     if (p.fill_tail) {
@@ -238,8 +254,17 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     if (x0 < x1) {
         uint32_t b = s_request;
         Kv4Request rq = kv4_request(p, b, Sh::kRows, false);
-        int item = (int)ratio_of(s_rest, rq.cells);          // tile * kv_heads + head
-        int c0 = (int)(s_rest - (long long)item * rq.cells), c1 = (int)min((long long)rq.cells, c0 + (x1 - x0));
+        const int unit = pieces ? kv4_pieces(rq.cells) : rq.cells;
+        int item = (int)ratio_of(s_rest, unit);              // tile * kv_heads + head
+        int c0 = (int)(s_rest - (long long)item * unit), c1;
+        if (pieces) {
+            const int piece = c0;
+            c0 = (int)((long long)piece * rq.cells / unit);
+            c1 = (int)((long long)(piece + 1) * rq.cells / unit);
+            x1 = x0 + (c1 - c0);
+        } else {
+            c1 = (int)min((long long)rq.cells, c0 + (x1 - x0));
+        }
         uint32_t head = (uint32_t)item % p.kv_heads;
         long long x = x0;
 
@@ -594,7 +619,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
             const int start = rq.start;
             const uint32_t at_head = head;
             if (!whole && !late) {                           // it ends in block (x + cells - 1) / per
-                cut.parts = (uint32_t)(ratio_of(x + rq.cells - 1, per) - blockIdx.x) + 1u;
+                cut.parts = pieces ? (uint32_t)kv4_pieces(rq.cells) : (uint32_t)(ratio_of(x + rq.cells - 1, per) - blockIdx.x) + 1u;
                 cut.row0 = (uint32_t)row0; cut.head = head; cut.start = (uint32_t)start; cut.rows = (uint32_t)all_rows;
             }
             x += c1 - c0;
