@@ -684,7 +684,7 @@ template <int D, int GS, int DT> cudaError_t run_chunk(const Kv4Attn& p, uint32_
         ready[dev] = true;
     }
     if (cudaError_t e = launch_early(kv4_chunk_kernel<D, GS, DT>, dim3(blocks), dim3(kChunkThreads), ChunkShape<D>::kBytes, s, p)) return e;
-    return launch_early(kv4_join_kernel<D, kChunkRows / 8, DT>, dim3(blocks, 16), dim3(128), 0, s, p, blocks);
+    return launch_early(kv4_join_kernel<D, kChunkRows / 8, DT>, dim3(blocks, 8), dim3(JoinShape<D>::kThreads), 0, s, p, blocks);
 }
 
 }  // namespace dd

@@ -150,6 +150,10 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4Attn& p, uint32_t b, 
 // 7.3 / 11.4, 777 tokens 9.7 / 12.5, 3000 tokens 10.3 / 12.9.
 __host__ __device__ constexpr int kv4_pieces(int cells) { return cells <= 16 ? 1 : (cells + 7) / 8; }
 
+// What the beginning and the end of a segment (queries, first cells, adding the warps' sums) cost a block, in cells: about 5500 cycles at 290 a
+// cell.  Without it blocks of short requests took half as long again as the others (64 requests of 512 to 16384 tokens: 112 us, with it WITH).
+constexpr int kSegmentCells = 16;
+
 template <int D, int NT> struct DecodeShape {
     static constexpr int kRows = 8 * NT;
     static constexpr int kRowStride = D + 4;            // floats; keeps the warps' 16-byte stores apart by banks
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     long long mine[2] = {0, 0};                                // cells, pieces
     for (uint32_t b = rb0; b < rb1; ++b) {
         const Kv4Request r = kv4_request(p, b, Sh::kRows, blockIdx.x == 0);
-        mine[0] += (long long)r.tiles * p.kv_heads * r.cells;
+        mine[0] += (long long)r.tiles * p.kv_heads * (r.cells + kSegmentCells);
         mine[1] += (long long)r.tiles * p.kv_heads * kv4_pieces(r.cells);
     }
     long long incl[2] = {mine[0], mine[1]};
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
             uint32_t b = rb0;
             for (;; ++b) {                                   // ends: x0 lies below the end of this run
                 const Kv4Request r = kv4_request(p, b, Sh::kRows, false);
-                const long long n = (long long)r.tiles * p.kv_heads * (kind ? kv4_pieces(r.cells) : r.cells);
+                const long long n = (long long)r.tiles * p.kv_heads * (kind ? kv4_pieces(r.cells) : r.cells + kSegmentCells);
                 if (x0 < at + n) break;
                 at += n;
             }
@@ -254,19 +258,18 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     if (x0 < x1) {
         uint32_t b = s_request;
         Kv4Request rq = kv4_request(p, b, Sh::kRows, false);
-        const int unit = pieces ? kv4_pieces(rq.cells) : rq.cells;
+        int unit = pieces ? kv4_pieces(rq.cells) : rq.cells + kSegmentCells;
         int item = (int)ratio_of(s_rest, unit);              // tile * kv_heads + head
-        int c0 = (int)(s_rest - (long long)item * unit), c1;
-        if (pieces) {
-            const int piece = c0;
-            c0 = (int)((long long)piece * rq.cells / unit);
-            c1 = (int)((long long)(piece + 1) * rq.cells / unit);
-            x1 = x0 + (c1 - c0);
-        } else {
-            c1 = (int)min((long long)rq.cells, c0 + (x1 - x0));
-        }
+        int pos = (int)(s_rest - (long long)item * unit);    // in the segment's part of the line: kSegmentCells for its beginning and end, its cells
         uint32_t head = (uint32_t)item % p.kv_heads;
         long long x = x0;
+        int take, c0, c1;                                    // of the line; cells
+        auto range = [&] {
+            take = (int)min((long long)(unit - pos), x1 - x);
+            c0 = pieces ? (int)((long long)pos * rq.cells / unit) : max(pos - kSegmentCells, 0);
+            c1 = pieces ? (int)((long long)(pos + take) * rq.cells / unit) : max(pos + take - kSegmentCells, 0);
+        };
+        range();
 
         // ---- this warp's steps of a segment: cells c0 + 2 (warp + 4 j), + 1
         int count;
@@ -303,8 +306,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
 #pragma unroll
             for (int j = 0; j < kStages - 1; ++j) issue(j);
         };
-        begin();
-        while (x < x1) {
+        if (c1 > c0) begin();
+        while (x < x1 && c1 > c0) {                          // a range that ends before the first cell of its last segment leaves that to the next
             const int row0 = (int)((uint32_t)item / p.kv_heads) * Sh::kRows;
             const int all_rows = rq.queries * (int)p.ratio;
 
@@ -618,20 +621,21 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
             const bool whole = c0 == 0 && c1 == rq.cells, late = c0 > 0;
             const int start = rq.start;
             const uint32_t at_head = head;
-            if (!whole && !late) {                           // it ends in block (x + cells - 1) / per
-                cut.parts = pieces ? (uint32_t)kv4_pieces(rq.cells) : (uint32_t)(ratio_of(x + rq.cells - 1, per) - blockIdx.x) + 1u;
+            if (!whole && !late) {                           // it ends in the block that has the segment's last place on the line
+                cut.parts = pieces ? (uint32_t)kv4_pieces(rq.cells) : (uint32_t)(ratio_of(x - pos + unit - 1, per) - blockIdx.x) + 1u;
                 cut.row0 = (uint32_t)row0; cut.head = head; cut.start = (uint32_t)start; cut.rows = (uint32_t)all_rows;
             }
-            x += c1 - c0;
+            x += take;
             if (x < x1) {
                 if (++item == rq.tiles * (int)p.kv_heads) {
                     item = 0;
                     do rq = kv4_request(p, ++b, Sh::kRows, false); while (rq.tiles == 0);      // ends: cells remain
                 }
-                c0 = 0;
-                c1 = (int)min((long long)rq.cells, x1 - x);
+                unit = rq.cells + kSegmentCells;             // a piece is a block's only one
+                pos = 0;
                 head = (uint32_t)item % p.kv_heads;
-                begin();
+                range();
+                if (c1 > c0) begin();
             }
 
             // ---- the warps' sums into shared memory
@@ -707,33 +711,40 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
     if (tid == 0) cuts[blockIdx.x] = cut;
 }
 
-// Adds the parts of a cut segment: blocks (block that began one, row of the tile modulo gridDim.y).
+// Adds the parts of a cut segment: a block takes four rows of it, and four parts of a row at the same time (two for heads of 256).  Few
+// blocks, since most cut segments have two or three parts and a block waits three round trips for them: one block a row took 30 us behind
+// 64 requests.
+constexpr int kJoinRows = 4;
+template <int D> struct JoinShape {
+    static constexpr int kLanes = D / 4, kWays = D == 256 ? 2 : 4, kThreads = kLanes * kWays * kJoinRows;
+};
+
 template <int D, int NT, int DT>
-__global__ void __launch_bounds__(128) kv4_join_kernel(Kv4Attn p, uint32_t blocks) {
+__global__ void __launch_bounds__(JoinShape<D>::kThreads) kv4_join_kernel(Kv4Attn p, uint32_t blocks) {
     using T = typename Tr<DT>::T;
-    constexpr int LANES = D / 4;                     // threads across a row
-    constexpr int WAYS = 128 / LANES;                // parts taken at the same time
-    __shared__ float4 s_v[WAYS][LANES];
-    __shared__ float s_ml[WAYS][2];
+    constexpr uint32_t LANES = JoinShape<D>::kLanes, WAYS = JoinShape<D>::kWays;
+    __shared__ float4 s_v[kJoinRows][WAYS][LANES];
+    __shared__ float s_ml[kJoinRows][WAYS][2];
     pdl_trigger();
     pdl_wait();
     const Kv4Cut cut = reinterpret_cast<const Kv4Cut*>(p.part + (size_t)blocks * 2u * kv4_part_floats(D, NT))[blockIdx.x];
     if (cut.parts == 0) return;
     const float* base = p.part + (size_t)blockIdx.x * 2u * kv4_part_floats(D, NT);
-    const uint32_t way = threadIdx.x / LANES, d4 = threadIdx.x % LANES;
-    for (uint32_t r = blockIdx.y; r < 8 * NT && cut.row0 + r < cut.rows; r += gridDim.y) {
-        const uint32_t row = cut.row0 + r;
+    const uint32_t d4 = threadIdx.x % LANES, way = threadIdx.x / LANES % WAYS, mine = threadIdx.x / (LANES * WAYS);
+    for (uint32_t r0 = blockIdx.y * kJoinRows; r0 < 8 * NT && cut.row0 + r0 < cut.rows; r0 += gridDim.y * kJoinRows) {
+        const uint32_t r = r0 + mine, row = cut.row0 + r;
+        const bool live = row < cut.rows;
         float top = -INFINITY, sum = 0.0f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         auto add = [&](float m, float l, const float4& o) {
-            if (m == -INFINITY && l == 0.0f) return;                          // saw nothing
+            if (m == -INFINITY && l == 0.0f) return;                      // saw nothing
             const float to = fmaxf(top, m), f0 = top == to ? 1.0f : ex2(top - to), f1 = m == to ? 1.0f : ex2(m - to);
             top = to;
             sum = sum * f0 + l * f1;
             v.x = v.x * f0 + o.x * f1; v.y = v.y * f0 + o.y * f1; v.z = v.z * f0 + o.z * f1; v.w = v.w * f0 + o.w * f1;
         };
-        constexpr uint32_t U = 8;                                             // parts that a thread has under way
-        for (uint32_t i0 = way; i0 < cut.parts; i0 += WAYS * U) {
+        constexpr uint32_t U = 4;                                         // parts that a thread has under way
+        for (uint32_t i0 = way; live && i0 < cut.parts; i0 += WAYS * U) {
             float2 ml[U];
             float4 o[U];
 #pragma unroll
@@ -750,12 +761,12 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(Kv4Attn p, uint32_t block
 #pragma unroll
             for (uint32_t k = 0; k < U; ++k) add(ml[k].x, ml[k].y, o[k]);
         }
-        s_v[way][d4] = v;
-        if (d4 == 0) { s_ml[way][0] = top; s_ml[way][1] = sum; }
+        s_v[mine][way][d4] = v;
+        if (d4 == 0) { s_ml[mine][way][0] = top; s_ml[mine][way][1] = sum; }
         __syncthreads();
-        if (way == 0) {
+        if (way == 0 && live) {
 #pragma unroll
-            for (int w = 1; w < WAYS; ++w) add(s_ml[w][0], s_ml[w][1], s_v[w][d4]);
+            for (uint32_t w = 1; w < WAYS; ++w) add(s_ml[mine][w][0], s_ml[mine][w][1], s_v[mine][w][d4]);
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const long long tok = cut.start + row / p.ratio, h = cut.head * p.ratio + row % p.ratio;
             T* dst = reinterpret_cast<T*>(p.out) + tok * p.out_token + h * p.out_head + 4 * d4;
@@ -763,7 +774,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(Kv4Attn p, uint32_t block
             *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
             if (p.lse && d4 == 0) p.lse[(size_t)tok * p.kv_heads * p.ratio + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
         }
-        __syncthreads();                                                  // the sums in shared memory are the next row's
+        __syncthreads();                                                  // the sums in shared memory are the next rows'
     }
 }
 
@@ -786,7 +797,7 @@ template <int D, int GS, int NT, int DT> int decode_blocks_per_sm() {
 template <int D, int GS, int NT, int DT> cudaError_t run_decode(const Kv4Attn& p, uint32_t blocks, cudaStream_t s) {
     if (!decode_blocks_per_sm<D, GS, NT, DT>()) return cudaErrorInvalidConfiguration;
     if (cudaError_t e = launch_early(kv4_decode_kernel<D, GS, NT, DT>, dim3(blocks), dim3(kDecodeThreads), decode_smem<D, GS, NT>(), s, p)) return e;
-    return launch_early(kv4_join_kernel<D, NT, DT>, dim3(blocks, 8 * NT), dim3(128), 0, s, p, blocks);
+    return launch_early(kv4_join_kernel<D, NT, DT>, dim3(blocks, 8 * NT / kJoinRows), dim3(JoinShape<D>::kThreads), 0, s, p, blocks);
 }
 
 // f<GS, NT, DT>() of a head size

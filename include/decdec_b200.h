@@ -64,8 +64,8 @@ int decdec_compiled_arch(void);
  * dec_config.cu:204-208).  Every wait inside the kernels of this library is bounded; a thread block that gives up
  * stores a code into the error word of the (device, stream) workspace: 1 = a wait for a shared-memory stage ran
  * out (DECDEC_PIPE_WAIT_NS, default 50 ms), 2 = the launch did not get the shared-memory layout it was sized for,
- * 3 = a call on the 4-bit key/value cache met a page or a slot outside the cache, or a length beyond its block table (it reads zeros there
- * and writes nothing).
+ * 3 = a call on the 4-bit key/value cache met a page or a slot outside the cache, or a length beyond its block table (it neither reads nor
+ * writes there).
  * The output of that launch is then incomplete.  The word lives in mapped host memory, so every later compute call
  * on that stream sees it without a copy and fails with DECDEC_E_DEVICE until the stream is reset.
  *   decdec_stream_status  *error_out = the word (0 = fine); does not synchronise.
