@@ -150,9 +150,10 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4Attn& p, uint32_t b, 
 // 7.3 / 11.4, 777 tokens 9.7 / 12.5, 3000 tokens 10.3 / 12.9.
 __host__ __device__ constexpr int kv4_pieces(int cells) { return cells <= 16 ? 1 : (cells + 7) / 8; }
 
-// What the beginning and the end of a segment (queries, first cells, adding the warps' sums) cost a block, in cells: about 5500 cycles at 290 a
-// cell.  Without it blocks of short requests took half as long again as the others (64 requests of 512 to 16384 tokens: 112 us, with it WITH).
-constexpr int kSegmentCells = 16;
+// What the beginning and the end of a segment (queries, first cells, adding the warps' sums) cost a block, in cells: 5 to 10 thousand cycles
+// at 290 a cell.  Counted as 0 / 16 / 32 / 48 cells: 64 requests of 512 to 16384 tokens 112 / 93 / 84 / 86 us, drafts of 17 requests 104 / 69 / 61
+// / 63: without it the blocks that have the short requests take twice as long as the others.
+constexpr int kSegmentCells = 32;
 
 template <int D, int NT> struct DecodeShape {
     static constexpr int kRows = 8 * NT;
