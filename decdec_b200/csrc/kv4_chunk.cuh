@@ -4,7 +4,8 @@
 // Per tile and step of 128 tokens, S = Q K^T and O += P V with fp16 operands and fp32 sums in tensor memory.  Keys and values become
 // fp16 numbers on the way (offset + step * code in one rounding, 2^-11, as a gathered cache in 16 bits has; scaled by a power of two per
 // 32 tokens so that both 16-bit types fit), once for the 256 rows of a tile.  Bound by the products and the exponentials: for heads of 128, a step
-// of a tile is 2048 cycles of each.
+// of a tile is 2048 cycles of each; it takes 6100, most of it the chain maximum -> exponentials -> products of a group.  Three requests with
+// chunks of up to 2048 queries at up to 16384 tokens: 1.26 ms, 685 TFLOP/s.
 //
 // One block an SM, 17 warps:
 //   warps 0-3, 4-7   rows 0-127 and 128-255 of the tile, a thread a row: queries into shared memory; per step the row's maximum and sum,

@@ -16,6 +16,9 @@
 //               small weights become subnormal before they are 2^-23 of the largest
 //   the rest    (scores, running maximum and sum, the middles' part, sums over thread blocks) in fp32
 //
+// Bound by memory and the instructions alike: 390 cycles a cell of 2176 bytes (heads of 128, one group) and scheduler, where the copy rate
+// allows 354.  64 requests of 512 to 16384 tokens, 372 MB: 84 us, 4.4 TB/s.
+//
 // The work is a line of cells (16 tokens of one key head), request by request, and every thread block takes an equal part of it
 // (lengths are on the device: each block sums them itself); work that would not fill the device is cut by segments instead.  A warp streams its own cells through shared memory (cp.async, kStages
 // cells ahead) and keeps its own running maximum and sums; the four warps of a block are added where a segment (one request, head and
