@@ -5,7 +5,7 @@
 // fp16 numbers on the way (offset + step * code in one rounding, 2^-11, as a gathered cache in 16 bits has; scaled by a power of two per
 // 32 tokens so that both 16-bit types fit), once for the 256 rows of a tile.  Bound by the products and the exponentials: for heads of 128, a step
 // of a tile is 2048 cycles of each; it takes 6100, most of it the chain maximum -> exponentials -> products of a group.  Three requests with
-// chunks of up to 2048 queries at up to 16384 tokens: 1.26 ms, 685 TFLOP/s.
+// chunks of up to 2048 queries at up to 16384 tokens: 1.24 ms, 697 TFLOP/s.
 //
 // One block an SM, 17 warps:
 //   warps 0-3, 4-7   rows 0-127 and 128-255 of the tile, a thread a row: queries into shared memory; per step the row's maximum and sum,
@@ -29,6 +29,7 @@ namespace dd {
 
 constexpr int kChunkRows = 256, kChunkStep = 128, kChunkThreads = 17 * 32;
 constexpr float kChunkGrow = 8.0f;
+constexpr int kSegmentSteps = 2;              // what a segment's beginning and end count on the line, in steps (counted as none: 2 % slower)
 constexpr unsigned kErrWait = 1;
 
 struct ChunkRequest {
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
     const uint32_t rb0 = min(warp * run, p.requests), rb1 = min(rb0 + run, p.requests);
     auto total_of = [&](const ChunkRequest& r) {
         long long n = 0;
-        for (int t = lane; t < r.tiles; t += 32) n += chunk_tile(p, r, t).steps;
+        for (int t = lane; t < r.tiles; t += 32) n += chunk_tile(p, r, t).steps + kSegmentSteps;
 #pragma unroll
         for (int o = 16; o; o /= 2) n += __shfl_xor_sync(0xffffffffu, n, o);
         return n * p.kv_heads;
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
             at += n;
         }
         for (int t0 = 0;; t0 += 32) {                                            // ends: x0 lies below the end of the request
-            const int t = t0 + lane, steps = t < r.tiles ? chunk_tile(p, r, t).steps : 0;
+            const int t = t0 + lane, steps = t < r.tiles ? chunk_tile(p, r, t).steps + kSegmentSteps : 0;
             const long long n = (long long)steps * p.kv_heads;
             long long incl = n;
 #pragma unroll
@@ -264,21 +265,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
         uint32_t b;
         ChunkRequest r;
         ChunkTile t;
-        int tile, head, c0, c1;
+        int tile, head, c0, c1, pos, take;                                       // pos, take: of its part of the line
         long long x;
     } g;
+    auto range = [&] {
+        g.take = (int)min((long long)(g.t.steps + kSegmentSteps - g.pos), x1 - g.x);
+        g.c0 = max(g.pos - kSegmentSteps, 0);
+        g.c1 = max(g.pos + g.take - kSegmentSteps, 0);
+    };
     auto first = [&] {
         g.x = x0;
         if (x0 >= x1) return;
-        g.b = (uint32_t)s_seg[0]; g.tile = s_seg[1]; g.head = s_seg[2]; g.c0 = s_seg[3];
+        g.b = (uint32_t)s_seg[0]; g.tile = s_seg[1]; g.head = s_seg[2]; g.pos = s_seg[3];
         g.r = chunk_request(p, g.b, false);
         g.t = chunk_tile(p, g.r, g.tile);
-        g.c1 = (int)min((long long)g.t.steps, g.c0 + (x1 - x0));
+        range();
     };
     auto next = [&] {
-        g.x += g.c1 - g.c0;
+        g.x += g.take;
         if (g.x >= x1) return;
-        g.c0 = 0;
+        g.pos = 0;
         if (++g.head == (int)p.kv_heads) {
             g.head = 0;
             if (++g.tile == g.r.tiles) {
@@ -287,8 +293,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
             }
             g.t = chunk_tile(p, g.r, g.tile);
         }
-        g.c1 = (int)min((long long)g.t.steps, x1 - g.x);
+        range();
     };
+    // a range that ends before the first step of its last segment leaves that to the next block
+    auto more = [&] { return g.x < x1 && g.c1 > g.c0; };
     const uint32_t smem_s = smem_at(smem), smem_k = smem_s + Sh::kQ, smem_v = smem_k + 2 * Sh::kK;
 
     if (warp == 16) {
@@ -305,7 +313,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                 products_done(bar_s + 8 * grp);
                 bar_arrive(bar_s + 8 * grp);                                     // what the converting warps left for the rows is visible with it
             };
-            for (first(); g.x < x1; next()) {
+            for (first(); more(); next()) {
                 const uint32_t groups = g.t.n * (int)p.ratio > 128 ? 2u : 1u;
                 const int steps = g.c1 - g.c0;
                 bar_wait(bar_q, seg & 1u, gave_up, p.err);
@@ -378,7 +386,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
             return at % 4 == 0 ? q.x : at % 4 == 1 ? q.y : at % 4 == 2 ? q.z : q.w;
         };
         const uint32_t bar_full = values ? bar_v : bar_k, bar_free = values ? bar_vfree : bar_kfree;
-        for (first(); g.x < x1; next()) {
+        for (first(); more(); next()) {
             const int block0 = g.t.from + g.c0, steps = g.c1 - g.c0;
             Raw cur, ahead;
             int page = page_of(block0);
@@ -485,7 +493,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
         const uint32_t at_s = tmem + 2 * D + grp * 128u + lanes, at_o = tmem + grp * D + lanes;
         uint32_t step = 0, seg = 0, turn = 0;
         Kv4Cut cut = {};
-        for (first(); g.x < x1; next()) {
+        for (first(); more(); next()) {
             const int live_rows = g.t.n * (int)p.ratio, steps = g.c1 - g.c0;
             const bool active = grp == 0 || live_rows > 128, live = row < live_rows;
             const int query = g.t.q0 + (live ? row / (int)p.ratio : 0), sub = live ? row % (int)p.ratio : 0;
@@ -661,7 +669,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
             }
             tc_before();
             if (!whole && !late && row == 0) {
-                cut.parts = (uint32_t)(ratio_of(g.x + g.t.steps - 1, per) - blockIdx.x) + 1u;
+                cut.parts = (uint32_t)(ratio_of(g.x - g.pos + g.t.steps + kSegmentSteps - 1, per) - blockIdx.x) + 1u;
                 cut.row0 = (uint32_t)(g.t.q0 * (int)p.ratio); cut.head = (uint32_t)g.head; cut.start = (uint32_t)g.r.start;
                 cut.rows = (uint32_t)((g.t.q0 + g.t.n) * (int)p.ratio);
             }
