@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                 for (int k = 0; k < D / 16; ++k)
                     product(tmem + 2 * D + grp * 128u, a + (k / 4) * (kChunkRows * 8u) + (k % 4) * 2u, b + (k / 4) * (kChunkStep * 8u) + (k % 4) * 2u, shape_s, k > 0);
                 products_done(bar_s + 8 * grp);
-                bar_arrive(bar_s + 8 * grp);                                     // what the converting warps left for the rows is visible with it
+                bar_arrive(bar_s + 8 * grp);                                     // what the key warps left for the rows is visible with it
             };
             for (first(); more(); next()) {
                 const uint32_t groups = g.t.n * (int)p.ratio > 128 ? 2u : 1u;
@@ -543,6 +543,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                 if (!active) continue;
                 bar_wait(bar_s + 8 * grp, turn & 1u, gave_up, p.err);
                 ++turn;
+                // The scores wait for the keys alone: the values' exponents and marks are there with the values of the step.  Their stage is not
+                // filled again before this group has handed its weights over, so the phase cannot be missed.
+                bar_wait(bar_v + 8 * (step & 1u), (step >> 1) & 1u, gave_up, p.err);
                 tc_after();
                 if (any_live) {
                     const ChunkMeta& meta = s_meta[step & 3u];

@@ -616,3 +616,31 @@ def test_steps_of_a_layer(kv4, dtype, d, group, interleaved):
             at += m
         assert (result["out"][n:] == 0).all()
         lengths, left = p.lengths.clone(), p.free_count.clone()
+
+
+# ---- tiles over long contexts --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["rising", "falling", "saw"])
+def test_tiles_of_values_whose_size_moves_from_step_to_step(kv4, dtype, kind):
+    """More than 4096 tokens and several heads, cut over many thread blocks; the values of every 32 tokens have another power of two, so that
+    exponents of an earlier step, of another head or of nothing would show.  Some values are no numbers, before the window of most rows."""
+    lengths, queries = [4700, 333, 1500], [40, 1, 33]
+    b = Batch(kv4, lengths, queries, 8, 4, 128, 64, dtype, 64, 2100)
+    for v in b.v:
+        at = torch.arange(len(v)) // 32
+        last = len(v) // 32
+        e = {"rising": -(last - at) // 6, "falling": -(at // 6), "saw": -(at * 5 % 11)}[kind].clamp(min=-12)
+        v *= (2.0 ** e.double())[:, None, None].to(dtype)
+    b.fill()
+    out, lse = b.run(return_lse=True)
+    assert b.dense
+    b.check(out, lse)
+    for _ in range(5):
+        assert torch.equal(out, b.run())
+    window = 2000
+    b.v[0][4700 - 39 - window, 1, 7] = math.inf                        # seen by the first row alone
+    b.v[0][4700 - 20 - window, 2, 70] = math.nan                       # by the first twenty
+    b.fill()
+    out, lse = b.run(window=window, return_lse=True)
+    b.check(out, lse, window=window)
