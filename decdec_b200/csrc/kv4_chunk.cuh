@@ -362,6 +362,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
             const int tok = block * kChunkStep + (t & ~15);
             return tok < g.r.length ? p.table[(long long)g.b * p.table_stride + (uint32_t)tok / kCellTokens / p.page_cells] : -1;
         };
+        // Coherent loads past the first-level cache: this block may have become resident before an append that it waited for wrote these bytes,
+        // which loads of read-only memory do not allow.
         auto load = [&](Raw& x, int page, int block) {
             const uint32_t r = t & 15, c = (uint32_t)(block * kChunkStep + t) / kCellTokens;
 #pragma unroll
@@ -374,11 +376,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
             }
             const uint8_t* cell = p.cache + ((size_t)page * p.kv_heads + g.head) * p.page_bytes + (size_t)(c % p.page_cells) * CELL;
 #pragma unroll
-            for (int i = 0; i < LW; ++i) x.x[i] = __ldg(reinterpret_cast<const uint4*>(cell + (values ? 8 * D : 0) + r * (D / 2)) + i);
+            for (int i = 0; i < LW; ++i) x.x[i] = __ldcg(reinterpret_cast<const uint4*>(cell + (values ? 8 * D : 0) + r * (D / 2)) + i);
             if (block * kChunkStep + t < g.r.length) {                           // else what the page held before
 #pragma unroll
                 for (int i = 0; i < NG; ++i)
-                    x.s[i] = __ldg(reinterpret_cast<const uint32_t*>(cell + (values ? kv4_value_step(D, GS, r, i) : kv4_key_step(D, GS, r, i))));
+                    x.s[i] = __ldcg(reinterpret_cast<const uint32_t*>(cell + (values ? kv4_value_step(D, GS, r, i) : kv4_key_step(D, GS, r, i))));
             }
         };
         auto word = [](const Raw& x, int at) {

@@ -566,6 +566,31 @@ def test_captured_and_replayed_beside_other_streams(kv4):
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(third, want[2])
 
 
+@pytest.mark.parametrize("queries", [1, 40])
+def test_rows_appended_just_before_they_are_read(kv4, queries):
+    """Launches begin while the call before them ends: new rows over ones that a gather and the attention before have read, without a pause."""
+    lengths = [600, 131, 64]
+    batches = [Batch(kv4, lengths, [queries] * 3, 8, 2, 128, 32, torch.float16, 16, 1100) for _ in range(2)]
+    batches[1].k, batches[1].v = [x.flip(0) for x in batches[0].k], [x * -2 for x in batches[0].v]
+    rows = [[torch.cat(x).cuda() for x in (b.k, b.v)] for b in batches]
+    slots, cache = torch.cat(batches[0].slots).cuda(), batches[0].cache
+    args = (batches[0].q.cuda(), cache, batches[0].table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), batches[0].starts.cuda(), 32)
+
+    def turn(i, pause):
+        held = kv4.gather(cache, slots, 128, 32, torch.float16)
+        pause()
+        kv4.append(cache, *rows[i], slots, 32)
+        pause()
+        return held + (kv4.attention(*args, max_queries=queries),)
+
+    want = [turn(i % 2, torch.cuda.synchronize) for i in range(4)][2:]
+    torch.cuda.synchronize()
+    got = [turn(i % 2, lambda: None) for i in range(40)]
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(x, want[i % 2])), i
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
