@@ -561,7 +561,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                     for (int c = 0; c < 4; ++c) {
                         uint32_t r[32];
                         tmem_load32(at_s + 32 * c, r);
-                        const float f = sf * pow2(meta.key_exp[c] - 12);
+                        // above 0, or a hidden score of -inf times 0 would be NaN: keys of zeros (parts of a step without tokens) have the least exponent
+                        const float f = fmaxf(sf * pow2(meta.key_exp[c] - 12), kLeastFactor);
                         // weights times 2^(exponent of the values here - that of the sums)
                         const int shift = max(meta.value_exp[c] - new_ev, -126);
                         tmem_loaded();

@@ -32,6 +32,9 @@ constexpr int kDecodeThreads = 128;
 constexpr int kDecodeWarps = 4;
 constexpr uint32_t kNoCell = 0xffffffffu;
 constexpr float kGrow = 4.0f;          // a running maximum follows once it is 2^4 behind
+// Factors of the scores stay above 0, where a hidden score of -inf would become NaN.  A score is then off by 2^-104 times the largest element
+// of the keys here (sums of 256 products with queries below 2^14), by 2^-92 in the tiles, whose keys are scaled too.
+constexpr float kLeastFactor = 1.17549435e-38f;
 
 // one part of a cut segment: [rows of a tile][D] sums, then [rows][2] maximum (log2 units) and sum
 __host__ __device__ constexpr uint32_t kv4_part_floats(uint32_t d, uint32_t nt) { return 8u * nt * (d + 2u); }
@@ -375,7 +378,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
                     sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
                     sum[g] *= 16.0f;
                 }
-                const float mine_sf = p.scale_log2 * pow2(e - 13);             // the sums with codes are 16 times too large
+                const float mine_sf = fmaxf(p.scale_log2 * pow2(e - 13), kLeastFactor);      // the sums with codes are 16 times too large
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     sf[nt][i] = __shfl_sync(0xffffffffu, mine_sf, 8 * tig + 4 * i);

@@ -591,6 +591,16 @@ def test_rows_appended_just_before_they_are_read(kv4, queries):
         assert all(torch.equal(a, b) for a, b in zip(x, want[i % 2])), i
 
 
+@pytest.mark.parametrize("queries", [1, 40])
+@pytest.mark.parametrize("dtype,size,scale", [(torch.bfloat16, -30, None), (torch.float16, -23, None), (torch.bfloat16, -100, None), (torch.bfloat16, -60, 1e-30)])
+def test_attention_of_small_queries(kv4, queries, dtype, size, scale):
+    """Queries and scales whose product with the factors of keys lies below the fp32 range, at lengths that leave parts of a step without tokens."""
+    b = Batch(kv4, [300, 64, 130], [queries] * 3, 8, 2, 128, 64, dtype, 16, 1200)
+    b.q *= 2.0 ** size
+    out, lse = b.run(return_lse=True, scale=scale)
+    b.check(out, lse, scale=scale)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
