@@ -563,8 +563,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                         tmem_load32(at_s + 32 * c, r);
                         // above 0, or a hidden score of -inf times 0 would be NaN: keys of zeros (parts of a step without tokens) have the least exponent
                         const float f = fmaxf(sf * pow2(meta.key_exp[c] - 12), kLeastFactor);
-                        // weights times 2^(exponent of the values here - that of the sums)
-                        const int shift = max(meta.value_exp[c] - new_ev, -126);
+                        // Weights times 2^(exponent of the values here - that of the sums).  Below -40 all of them (2^8 at most) are zeros in fp16 as
+                        // well, and the sum, which is taken before that rounding, must not lose them: it keeps those above 2^-86.
+                        const int shift = max(meta.value_exp[c] - new_ev, -40);
                         tmem_loaded();
                         if (!clear) {
                             const int lo = max(from - (tok0 + 32 * c), 0), hi = min(to - (tok0 + 32 * c), 32);

@@ -601,6 +601,27 @@ def test_attention_of_small_queries(kv4, queries, dtype, size, scale):
     b.check(out, lse, scale=scale)
 
 
+def test_tokens_without_values_count_in_the_sum(kv4):
+    """One token in 129 has a value, 2^15, all others zeros and weights of 2^-11.5: together they are 4 % of the sum."""
+    n, far = 32 + 4096, 11.5
+    b = Batch(kv4, [n], [33], 2, 1, 128, 64, torch.float16, 64, 1300)
+    b.q.zero_()
+    b.q[:, :, 0] = 1
+    b.k[0].zero_()
+    b.k[0][:, :, 1::64] = 15                                           # steps of 1: the cache holds these keys and values exactly
+    b.k[0][:32, :, 0] = 9
+    b.v[0].zero_()
+    b.v[0][:32] = 2.0 ** 15
+    b.fill()
+    out, lse = b.run(scale=far * math.log(2.0) / 9, return_lse=True)
+    assert b.dense
+    for i in range(33):
+        total = 32 + (n - 32 - 32 + i) * 2.0 ** -far
+        # half an fp16 step of the weights and of the output; scores in 32 bits
+        assert ((out[i].double() / (2.0 ** 15 * 32 / total) - 1).abs() <= 2.0 ** -10 + 2.0 ** -16).all(), i
+        assert ((lse[i].double() - (math.log(total) + far * math.log(2.0))).abs() <= 2.0 ** -16).all(), i
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
