@@ -581,8 +581,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                         const bool follow = top > m + kChunkGrow || (c == 0 && j > 0 && new_ev != ev);
                         if (__any_sync(0xffffffffu, follow)) {
                             // rare after a segment's first steps: the sums, and the weights of the step that are written already, brought to
-                            // another maximum or exponent
-                            const float now = fmaxf(m, top), down = m == now ? 1.0f : ex2(m - now), by = down * ex2((float)((j > 0 && c == 0 ? ev : new_ev) - new_ev));
+                            // another maximum or exponent.  Maxima are whole numbers, so that this is by powers of two: the fp16 weights of the step
+                            // lose nothing by it but what becomes subnormal.
+                            const float now = ceilf(fmaxf(m, top)), down = m == now ? 1.0f : m - now < -126.0f ? 0.0f : pow2((int)(m - now));
+                            const float by = down * ex2((float)((j > 0 && c == 0 ? ev : new_ev) - new_ev));
                             m = now;
                             l *= down;
                             tmem_stored();

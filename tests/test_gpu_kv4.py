@@ -622,6 +622,27 @@ def test_tokens_without_values_count_in_the_sum(kv4):
         assert ((lse[i].double() - (math.log(total) + far * math.log(2.0))).abs() <= 2.0 ** -16).all(), i
 
 
+def test_weights_keep_their_bits_when_a_maximum_moves_within_a_step(kv4):
+    """Every 32 tokens the largest score of a row grows by a factor 0.5 (1 + 0.9 * 2^-11) of its weights, whose rounding to fp16 is as large as can be, and
+    that of the row beside it by 2^16, so that the sums of both are brought to another maximum four times in a step."""
+    grow = 1 - math.log2(1 + 0.9 * 2.0 ** -11)
+    b = Batch(kv4, [128], [33], 2, 1, 128, 64, torch.float16, 16, 1400)
+    b.q.zero_()
+    b.q[:, 0, 0], b.q[:, 1, 0] = 1, 16
+    b.k[0].zero_()
+    b.k[0][:, :, 1::64] = 15                                           # steps of 1, and of 1/16 for the values: held exactly
+    b.k[0][:, 0, 0] = torch.arange(128) // 32
+    b.v[0].zero_()
+    b.v[0][:32] = 1 + (torch.arange(128) % 16) / 16
+    b.fill()
+    out = b.run(scale=grow * math.log(2.0))
+    assert b.dense
+    w = 2.0 ** (grow * (torch.arange(128) // 32).double())
+    want = (w @ b.v[0][:, 0].double()) / w.sum()
+    # half an fp16 step of the weights and of the output; scores in 32 bits
+    assert ((out[32, 0].cpu().double() - want).abs() <= (2.0 ** -10 + 2.0 ** -16) * want).all()
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
