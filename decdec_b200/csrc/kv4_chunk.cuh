@@ -406,10 +406,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
                     const float2 f = unpack2<DT>(cur.s[i]);
-                    const float m = fmaxf(fabsf(f.y), fabsf(fmaf(15.0f, f.x, f.y)));
-                    if (m < INFINITY) top = fmaxf(top, m);
+                    const float m = fmaxf(fabsf(f.y), fabsf(fmaf(15.0f, f.x, f.y)));        // a rounded step may lead beyond the largest number
+                    if (fabsf(f.y) < INFINITY) top = fmaxf(top, fminf(m, 3.402823466e+38f));
                 }
-                int e = min(max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127, -100), 120);
+                int e = max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127, -100);
                 ChunkMeta& meta = s_meta[step & 3u];
                 if (!values) {
                     if (lane == 0) meta.key_exp[w4] = e;

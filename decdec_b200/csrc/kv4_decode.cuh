@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(steps[g], 0.0f)));
-                        const int e = min(max((int)(bits >> 23) - 127, -100), 100);   // the largest step is below 2^(e+1)
+                        const int e = min(max((int)(bits >> 23) - 127, -100), 127);   // the largest step is below 2^(e+1)
                         const float want = pow2(10 - e);
                         float by = 1.0f;
                         if (limit[g] < 0.0f || want < fv[g]) {

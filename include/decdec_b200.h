@@ -227,6 +227,8 @@ int decdec_dummy_sqllm(const void* x_dev, void* y_dev, const int32_t* qweight, c
  *                       row that sees nothing gives zeros (lse -inf).  max_queries bounds the rows of a request and chooses the kernel;
  *                       requests with more are computed all the same.  Rows behind the last request stay as they are, or are cleared if
  *                       clear_tail.  lse, if not null: fp32 [rows][heads], the logarithm of the sum of exp(scaled scores).
+ *                       Scores and sums are fp32: keys beyond 2^100, or values whose sum weighted by up to 2^8 a token passes 2^128, may come out
+ *                       as infinities or NaN.
  *                       The workspace (bytes from _workspace, 16-byte aligned) holds nothing between calls; calls that may overlap in time
  *                       need one each. */
 int decdec_rotary(const void* q, int64_t q_token, int64_t q_head, uint32_t q_heads, const void* k, int64_t k_token, int64_t k_head, uint32_t k_heads,

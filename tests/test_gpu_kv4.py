@@ -643,6 +643,21 @@ def test_weights_keep_their_bits_when_a_maximum_moves_within_a_step(kv4):
     assert ((out[32, 0].cpu().double() - want).abs() <= (2.0 ** -10 + 2.0 ** -16) * want).all()
 
 
+@pytest.mark.parametrize("queries,keys,values", [(1, 0, 114), (40, 0, 125), (40, 123, 0), (1, 98, 0)])
+def test_attention_of_large_bf16_numbers(kv4, queries, keys, values):
+    """Values whose weighted sums, and keys whose scores, still fit 32 bits."""
+    b = Batch(kv4, [70, 20], [queries, 1], 8, 2, 128, 64, torch.bfloat16, 16, 1500)
+    for k, v in zip(b.k, b.v):
+        k *= 2.0 ** keys
+        v *= 2.0 ** values
+    b.q *= 2.0 ** -min(keys, 98)
+    b.fill()
+    scale = 2.0 ** (min(keys, 98) - keys) * 128 ** -0.5
+    out, lse = b.run(return_lse=True, max_queries=queries, scale=scale)
+    assert torch.isfinite(out).all()
+    b.check(out, lse, scale=scale)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
