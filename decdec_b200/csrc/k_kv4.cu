@@ -237,13 +237,25 @@ __device__ __forceinline__ float exact_code(float xh, float loh, float steph, fl
     return fminf(fmaxf(n, 0.0f), 15.0f);
 }
 
-// (hi - lo) / 15 rounded to the type, of halves.  The quotient by a constant is corrected by its remainder, which rounds as a division does
-// (Markstein's theorem) where nothing underflows.
+// (hi - lo) / 15 rounded to the type as over the reals, of halves.  The quotient by a constant is corrected by its remainder, which rounds as
+// a division does (Markstein's theorem) where nothing underflows: it is off by less than two units of 32 bits.  That is too much only next to
+// the middle of two numbers of the type.  15 times a middle is an odd multiple of a 2^12th (fp16; bf16: 2^9th) of the step's power of two, so the
+// range comes that near without meeting it only by a small end of the group whose own last bit lies 2^-25 below the range: fp16 alone has such
+// (bf16: 2^-19), and no subnormal steps, whose ranges are whole multiples of 2^-24.  There the range is compared with 15 middles exactly.
 template <int DT> __device__ __forceinline__ float step_of(float lo, float hi) {
-    const float range = 0.5f * hi - 0.5f * lo;
+    const float a = 0.5f * hi, b = 0.5f * lo, range = a - b;
     float q = range * (1.0f / 7.5f);
     q = fmaf(fmaf(-q, 7.5f, range), 1.0f / 7.5f, q);
     if (range < 1e-30f) q = range / 7.5f;
+    if constexpr (DT == FP16) {
+        const uint32_t bits = __float_as_uint(q);
+        if ((bits & 0x1fffu) - 0xffcu <= 8u) {                       // of the 13 bits that fp16 leaves off; about one group in 2^10
+            const uint32_t middle = (bits & ~0x1fffu) | 0x1000u;
+            const float back = range + b, e = (a - back) + ((back - range) - b);      // a - b = range + e
+            const float over = fmaf(-7.5f, __uint_as_float(middle), range) + e;
+            q = __uint_as_float(middle + (over > 0.0f) - (over < 0.0f));
+        }
+    }
     return Tr<DT>::to_f(Tr<DT>::from_f(q));
 }
 

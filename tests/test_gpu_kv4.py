@@ -658,6 +658,50 @@ def test_attention_of_large_bf16_numbers(kv4, queries, keys, values):
     b.check(out, lse, scale=scale)
 
 
+def test_steps_next_to_the_middle_of_two_numbers(kv4):
+    """(largest - least) / 15 a hair above, on and below the middle of two fp16 numbers: rounded as over the reals, ties to even."""
+    from fractions import Fraction
+
+    def to_half(x):                                                    # a positive number in the normal range
+        e = 0
+        while x >= Fraction(2) ** (e + 1):
+            e += 1
+        while x < Fraction(2) ** e:
+            e -= 1
+        n, unit = x / Fraction(2) ** (e - 10), Fraction(2) ** (e - 10)
+        whole = n.numerator // n.denominator
+        rest = n - whole
+        return (whole + (rest > Fraction(1, 2) or (rest == Fraction(1, 2) and whole % 2 == 1))) * unit
+
+    rng = np.random.RandomState(22)
+    groups, want = [], []
+    while len(groups) < 2048:
+        e = int(rng.randint(-12, 8))
+        span = 15 * Fraction(2 * int(rng.randint(1024, 2048)) + 1) * Fraction(2) ** (e - 11)         # 15 times a middle
+        if span >= 65504:
+            continue
+        hi = Fraction(float(np.float16(float(span))))
+        lo = float(hi - span)
+        if Fraction(float(np.float16(lo))) != hi - span or lo == 0.0:
+            continue
+        for least in (np.float16(lo), np.nextafter(np.float16(lo), np.float16(-1)), np.nextafter(np.float16(lo), np.float16(1))):
+            for sign in (1, -1):                                       # and mirrored
+                ends = (float(least), float(hi)) if sign == 1 else (-float(hi), -float(least))
+                groups.append(ends)
+                want.append(float(to_half((Fraction(ends[1]) - Fraction(ends[0])) / 15)))
+    groups.append((-3.0458e-05, 1.8671875))
+    lo = float(np.float16(-3.0458e-05))
+    want.append(float(to_half((Fraction(1.8671875) - Fraction(lo)) / 15)))
+    groups, want = groups[:len(groups) // 16 * 16], want[:len(groups) // 16 * 16]
+    x = torch.tensor(groups, dtype=torch.float64).repeat(1, 32).half().view(-1, 1, 64)       # one group of 64 a token
+    cache = kv4.empty_cache(len(x) // 16, 16, 1, 64, 64)
+    kv4.append(cache, x.cuda(), x.cuda(), torch.arange(len(x), device="cuda"), 64)
+    steps = cache.view(len(x) // 16, -1).cpu()[:, 16 * 64:].contiguous().view(torch.float16).view(len(x) // 16, 2, 16, 2)
+    for side in range(2):
+        assert torch.equal(steps[:, side, :, 0].flatten().double(), torch.tensor(want, dtype=torch.float64))
+        assert torch.equal(steps[:, side, :, 1].flatten(), x.amin(-1).flatten())
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
