@@ -77,7 +77,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
                 return rotary_dim * math.log(far / (turns * 2 * math.pi)) / (2 * math.log(base))
 
             lo = max(math.floor(pair(scaling.get("beta_fast", 32.0))), 0)
-            hi = min(math.ceil(pair(scaling.get("beta_slow", 1.0))), rotary_dim // 2 - 1)
+            hi = min(math.ceil(pair(scaling.get("beta_slow", 1.0))), rotary_dim - 1)
             slow = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0, 1)
             f = f * (1 - slow + slow / by)
             factor = float(scaling.get("attention_factor", 0.1 * math.log(by) + 1.0))

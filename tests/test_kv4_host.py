@@ -171,3 +171,16 @@ def test_restated_quantizer():
     assert step[1, 0] == 0 and lo[1, 0] == 2 and (code[1] == 0).all()
     assert math.isnan(lo[2, 0]) and math.isnan(lo[3, 0]) and step[2, 0] == 0
     assert torch.isnan(R.held(x, 32)[2:]).all()
+
+
+@pytest.mark.parametrize("length", [65536, 131072])
+def test_yarn_where_every_pair_turns_over_the_trained_length(kv4, length):
+    """The ramp's upper end lies behind the last pair when the trained length is above 2 pi base: it is cut at the rotated elements, not at their pairs."""
+    g, _ = kv4.rotary_frequencies(128, 10000.0, {"type": "yarn", "factor": 16.0, "original_max_position_embeddings": length}, device="cpu")
+    # pairs with 32 turns and one turn over the length: 128 ln(length / (2 pi turns)) / (2 ln 10000) = 40.2 and 64.3, 45.03 and 69.1
+    first, last = {65536: (40, 65), 131072: (45, 70)}[length]
+    for i in range(64):
+        slow = min(max((i - first) / (last - first), 0.0), 1.0)
+        want = 10000.0 ** (-i / 64) * (1 - slow + slow / 16)
+        assert abs(g[i].item() - want) <= 1e-13 * want, i
+    assert g[63].item() / 10000.0 ** (-63 / 64) > {65536: 0.13, 131072: 0.32}[length]
