@@ -75,7 +75,7 @@ int decdec_kv4_attention_workspace(uint32_t requests, uint32_t rows, uint32_t he
 int decdec_kv4_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t out_token, int64_t out_head, float* lse, const void* cache,
                          uint32_t pages, uint32_t page_size, const int32_t* table, int64_t table_stride, uint32_t table_cols, const int32_t* lengths,
                          const int32_t* query_starts, uint32_t requests, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
-                         uint32_t group_size, uint32_t max_queries, float scale, uint32_t window, int clear_tail, void* workspace,
+                         uint32_t group_size, uint32_t max_queries, float scale, uint32_t window, int clear_rest, void* workspace,
                          size_t workspace_bytes, int dtype, void* stream) {
     if (int r = check(requests, rows, heads, kv_heads, head_dim, group_size, max_queries, dtype)) return r;
     if (page_size == 0 || page_size % kCellTokens || page_size > 65536u)
@@ -107,7 +107,7 @@ int decdec_kv4_attention(const void* q, int64_t q_token, int64_t q_head, void* o
     p.requests = requests; p.rows = rows; p.kv_heads = kv_heads; p.ratio = ratio;
     p.window = window > 0x7fffffffu ? 0u : window;
     p.q_vec = (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && q_token % 8 == 0 && q_head % 8 == 0;
-    p.fill_tail = clear_tail ? 1u : 0u;
+    p.clear_rest = clear_rest ? 1u : 0u;
     p.scale_log2 = scale * 1.4426950408889634f;
     cudaError_t e;
     if (c.chunk) {

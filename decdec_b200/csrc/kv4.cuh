@@ -74,7 +74,7 @@ struct Kv4Attn {
     uint32_t requests, rows, kv_heads, ratio;
     uint32_t window;
     uint32_t q_vec;                       // queries may be read 16 bytes at a time
-    uint32_t fill_tail;                   // rows behind the last request are cleared
+    uint32_t clear_rest;                  // rows of no request are cleared
     float scale_log2;                     // scale of the scores * log2(e)
 };
 

@@ -250,15 +250,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
     __syncthreads();
     tc_after();
     const uint32_t tmem = s_tmem;
-    if (p.fill_tail) {
-        const int used = p.requests ? min(max(p.starts[p.requests], 0), (int)p.rows) : 0;
-        for (int t = used + (int)blockIdx.x; t < (int)p.rows; t += gridDim.x) {
-            for (uint32_t e = tid; e < p.kv_heads * p.ratio * D; e += kChunkThreads)
-                reinterpret_cast<T*>(p.out)[(long long)t * p.out_token + (long long)(e / D) * p.out_head + e % D] = Tr<DT>::from_f(0.0f);
-            if (p.lse)
-                for (uint32_t e = tid; e < p.kv_heads * p.ratio; e += kChunkThreads) p.lse[(size_t)t * p.kv_heads * p.ratio + e] = -INFINITY;
-        }
-    }
+    if (p.clear_rest) clear_rest<D, DT>(p, tid, kChunkThreads);
 
     // ---- the segments, walked by every warp for itself
     struct Segment {

@@ -161,6 +161,19 @@ __host__ __device__ constexpr int kv4_pieces(int cells) { return cells <= 16 ? 1
 // / 63: without it the blocks that have the short requests take twice as long as the others.
 constexpr int kSegmentCells = 32;
 
+// the rows before the first request and behind the last, a row a block at a time
+template <int D, int DT> __device__ __forceinline__ void clear_rest(const Kv4Attn& p, int tid, int threads) {
+    using T = typename Tr<DT>::T;
+    const int rows = (int)p.rows, first = p.requests ? min(max(p.starts[0], 0), rows) : 0, end = p.requests ? min(max(p.starts[p.requests], 0), rows) : 0;
+    for (long long i = blockIdx.x; i < (long long)first + (rows - end); i += gridDim.x) {
+        const int t = i < first ? (int)i : end + (int)(i - first);
+        for (uint32_t e = tid; e < p.kv_heads * p.ratio * D; e += threads)
+            reinterpret_cast<T*>(p.out)[(long long)t * p.out_token + (long long)(e / D) * p.out_head + e % D] = Tr<DT>::from_f(0.0f);
+        if (p.lse)
+            for (uint32_t e = tid; e < p.kv_heads * p.ratio; e += threads) p.lse[(size_t)t * p.kv_heads * p.ratio + e] = -INFINITY;
+    }
+}
+
 template <int D, int NT> struct DecodeShape {
     static constexpr int kRows = 8 * NT;
     static constexpr int kRowStride = D + 4;            // floats; keeps the warps' 16-byte stores apart by banks
@@ -252,15 +265,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_residency<D, GS, NT>())
         }
     }
     __syncthreads();
-    if (p.fill_tail) {
-        const int used = p.requests ? min(max(p.starts[p.requests], 0), (int)p.rows) : 0;
-        for (int t = used + (int)blockIdx.x; t < (int)p.rows; t += gridDim.x) {
-            for (uint32_t e = tid; e < p.kv_heads * p.ratio * D; e += kDecodeThreads)
-                reinterpret_cast<T*>(p.out)[(long long)t * p.out_token + (long long)(e / D) * p.out_head + e % D] = Tr<DT>::from_f(0.0f);
-            if (p.lse)
-                for (uint32_t e = tid; e < p.kv_heads * p.ratio; e += kDecodeThreads) p.lse[(size_t)t * p.kv_heads * p.ratio + e] = -INFINITY;
-        }
-    }
+    if (p.clear_rest) clear_rest<D, DT>(p, tid, kDecodeThreads);
     Kv4Cut cut = {};
     if (x0 < x1) {
         uint32_t b = s_request;

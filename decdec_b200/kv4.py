@@ -128,7 +128,7 @@ def attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, l
     head_dim], which are its last tokens, and lengths[b] tokens in the cache with them.  Query head h reads key head h * kv_heads // heads.
 
     window > 0: each row sees the last `window` tokens up to its own.  A row that sees no token gives zeros.  max_queries: the most rows of a
-    request (default: all rows), which chooses the kernel.  scale: default head_dim ** -0.5.  Rows behind the last request are left as
-    they are in `out`, zeros where `out` is not given.  return_lse: also the fp32 logarithms [tokens, heads] of the sums of exp(scale q k^T)."""
+    request (default: all rows), which chooses the kernel.  scale: default head_dim ** -0.5.  Rows of no request, before the first or
+    behind the last, are left as they are in `out`, zeros where `out` is not given.  return_lse: also the fp32 logarithms [tokens, heads] of the sums of exp(scale q k^T)."""
     out, lse = _kv4.attention(q, cache, block_table, lengths, query_starts, group_size, max_queries, scale, window, out, return_lse)
     return (out, lse) if return_lse else out

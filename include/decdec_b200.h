@@ -225,8 +225,8 @@ int decdec_dummy_sqllm(const void* x_dev, void* y_dev, const int32_t* qweight, c
  *                       rows query_starts[b] .. query_starts[b+1] - 1 and lengths[b] tokens in the cache, its own among them: row i stands
  *                       at position lengths[b] - queries + i and sees the tokens up to its own, the last `window` of them if window > 0.  A
  *                       row that sees nothing gives zeros (lse -inf).  max_queries bounds the rows of a request and chooses the kernel;
- *                       requests with more are computed all the same.  Rows behind the last request stay as they are, or are cleared if
- *                       clear_tail.  lse, if not null: fp32 [rows][heads], the logarithm of the sum of exp(scaled scores).
+ *                       requests with more are computed all the same.  Rows of no request (before the first, behind the last) stay as they are,
+ *                       or are cleared if clear_rest.  lse, if not null: fp32 [rows][heads], the logarithm of the sum of exp(scaled scores).
  *                       Scores and sums are fp32: keys beyond 2^100, or values whose sum weighted by up to 2^8 a token passes 2^128, may come out
  *                       as infinities or NaN.
  *                       The workspace (bytes from _workspace, 16-byte aligned) holds nothing between calls; calls that may overlap in time
@@ -249,7 +249,7 @@ int decdec_kv4_attention_workspace(uint32_t requests, uint32_t rows, uint32_t he
 int decdec_kv4_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t out_token, int64_t out_head, float* lse, const void* cache,
                          uint32_t pages, uint32_t page_size, const int32_t* table, int64_t table_stride, uint32_t table_cols, const int32_t* lengths,
                          const int32_t* query_starts, uint32_t requests, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
-                         uint32_t group_size, uint32_t max_queries, float scale, uint32_t window, int clear_tail, void* workspace,
+                         uint32_t group_size, uint32_t max_queries, float scale, uint32_t window, int clear_rest, void* workspace,
                          size_t workspace_bytes, int dtype, void* stream);
 
 #ifdef __cplusplus

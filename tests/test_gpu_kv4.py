@@ -702,6 +702,22 @@ def test_steps_next_to_the_middle_of_two_numbers(kv4):
         assert torch.equal(steps[:, side, :, 1].flatten(), x.amin(-1).flatten())
 
 
+@pytest.mark.parametrize("queries", [2, 40])
+def test_rows_before_the_first_request(kv4, queries):
+    """query_starts that do not begin at 0: the rows before are nobody's, zeros in a fresh output and left as they are in a given one."""
+    b = Batch(kv4, [50, 64], [queries, 1], 4, 2, 128, 128, torch.float16, 16, 810)
+    want = b.run(max_queries=queries)
+    q = torch.cat((torch.full((6, 4, 128), math.nan, dtype=torch.float16), b.q, torch.zeros(3, 4, 128, dtype=torch.float16))).cuda()
+    b.starts += 6
+    junk = [torch.full_like(q, 9.0) for _ in range(8)]                 # what a fresh output finds in its memory
+    del junk
+    out, lse = b.run(q=q, max_queries=queries, return_lse=True)
+    assert (out[:6] == 0).all() and (lse[:6] == -math.inf).all() and torch.equal(out[6:-3], want) and (out[-3:] == 0).all()
+    out = torch.full_like(q, 7.0)
+    b.run(q=q, max_queries=queries, out=out)
+    assert (out[:6] == 7).all() and torch.equal(out[6:-3], want) and (out[-3:] == 7).all()
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
