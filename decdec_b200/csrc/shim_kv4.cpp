@@ -48,27 +48,36 @@ void on_gpu(const Tensor& first, std::initializer_list<const Tensor*> others) {
 
 constexpr const char* kOverlap = "an output must not share memory with itself, another output or an input.";
 
-// rows [tokens][heads][d]: elements from the first to the last of a token
-int64_t extent(const Tensor& t) { return (t.size(1) - 1) * t.stride(1) + t.size(2); }
+// rows [tokens][heads][d]: elements from the first to the last of a token, of a head, of all
+int64_t token_extent(const Tensor& t) { return (t.size(1) - 1) * t.stride(1) + t.size(2); }
+int64_t head_extent(const Tensor& t) { return (t.size(0) - 1) * t.stride(0) + t.size(2); }
+int64_t extent(const Tensor& t) { return (t.size(0) - 1) * t.stride(0) + token_extent(t); }
 bool same(const Tensor& a, const Tensor& b) { return a.data_ptr() == b.data_ptr() && a.strides() == b.strides(); }
-// whether no two elements of t share a place (views whose heads or tokens are wound into one another count as sharing)
+// whether no two elements of t share a place: tokens one after another, or heads (views whose heads and tokens are wound into one another count as
+// sharing)
 bool spread(const Tensor& t) {
-    return t.numel() == 0 || ((t.size(1) == 1 || t.stride(1) >= t.size(2)) && (t.size(0) == 1 || t.stride(0) >= extent(t)));
+    if (t.numel() == 0) return true;
+    const bool one_token = t.size(0) == 1, one_head = t.size(1) == 1;
+    return ((one_head || t.stride(1) >= t.size(2)) && (one_token || t.stride(0) >= token_extent(t))) ||
+           ((one_token || t.stride(0) >= t.size(2)) && (one_head || t.stride(1) >= head_extent(t)));
 }
 // whether a and b share no place: ranges apart, or the same token stride and different parts of it (parts of a fused projection), or the
-// same head stride and different parts of that.  What it cannot tell counts as sharing.
+// same head stride and different parts of that; and the other way about for heads that hold all tokens.  What it cannot tell counts as sharing.
 bool apart(const Tensor& a, const Tensor& b) {
     if (!a.numel() || !b.numel()) return true;
     const int64_t size = a.element_size(), pa = (int64_t)a.data_ptr() / size, pb = (int64_t)b.data_ptr() / size;
-    const int64_t ea = extent(a), eb = extent(b), la = (a.size(0) - 1) * a.stride(0) + ea, lb = (b.size(0) - 1) * b.stride(0) + eb;
-    if (pa + la <= pb || pb + lb <= pa) return true;
+    if (pa + extent(a) <= pb || pb + extent(b) <= pa) return true;
     auto within = [&](int64_t period, int64_t na, int64_t nb) {
         if (period <= 0) return false;
         const int64_t d = ((pb - pa) % period + period) % period;
         return d >= na && d + nb <= period;
     };
-    if (a.stride(0) == b.stride(0) && within(a.stride(0), ea, eb)) return true;
-    return a.stride(1) == b.stride(1) && a.stride(0) == b.stride(0) && a.stride(1) > 0 && a.stride(0) % a.stride(1) == 0 && within(a.stride(1), a.size(2), b.size(2));
+    const bool token = a.stride(0) == b.stride(0), head = a.stride(1) == b.stride(1);
+    if (token && within(a.stride(0), token_extent(a), token_extent(b))) return true;
+    if (head && within(a.stride(1), head_extent(a), head_extent(b))) return true;
+    if (!token || !head) return false;
+    const int64_t inner = std::min(a.stride(0), a.stride(1)), outer = std::max(a.stride(0), a.stride(1));
+    return inner > 0 && outer % inner == 0 && within(inner, a.size(2), b.size(2));
 }
 
 const Tensor* at_or_null(const Maybe& t) { return t ? &*t : nullptr; }

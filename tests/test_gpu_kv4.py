@@ -718,6 +718,31 @@ def test_rows_before_the_first_request(kv4, queries):
     assert (out[:6] == 7).all() and torch.equal(out[6:-3], want) and (out[-3:] == 7).all()
 
 
+def test_outputs_with_heads_before_tokens(kv4):
+    """Queries, keys and outputs that are stored head by head, and rotary in place on them."""
+    frequencies, _ = kv4.rotary_frequencies(64)
+    q, k = normal((4, 7, 64), torch.float16, 44).cuda().transpose(0, 1), normal((2, 7, 64), torch.float16, 45).cuda().transpose(0, 1)
+    pos = torch.arange(7, device="cuda")
+    want = kv4.rotary(q.contiguous(), k.contiguous(), pos, frequencies)
+    out = torch.empty_like(q.contiguous().transpose(0, 1).contiguous()).transpose(0, 1), torch.empty((2, 9, 64), dtype=torch.float16, device="cuda")[:, 1:8].transpose(0, 1)
+    kv4.rotary(q, k, pos, frequencies, out=out)
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        kv4.rotary(q[:6], None, pos[:6], frequencies, out=(q[1:], None))
+    both = torch.cat((q, k), 1).transpose(0, 1).contiguous().transpose(0, 1)                 # queries and keys of one tensor, head by head
+    kv4.rotary(both[:, :4], both[:, 4:], pos, frequencies, out=(both[:, :4], both[:, 4:]))
+    assert torch.equal(both, torch.cat(want, 1))
+    kv4.rotary(q, k, pos, frequencies, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    b = Batch(kv4, [40], [7], 4, 2, 64, 64, torch.float16, 16, 672)
+    want = b.run()
+    out = torch.full((4, 8, 64), 7.0, dtype=torch.float16, device="cuda")
+    b.run(out=out[:, :7].transpose(0, 1))
+    assert torch.equal(out[:, :7].transpose(0, 1), want) and (out[:, 7] == 7).all()
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        b.run(out=out.flatten()[:448 + 64].as_strided((7, 4, 64), (64, 64, 1)))              # heads that lie over the tokens
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
