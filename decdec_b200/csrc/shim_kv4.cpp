@@ -80,6 +80,23 @@ bool apart(const Tensor& a, const Tensor& b) {
     return inner > 0 && outer % inner == 0 && within(inner, a.size(2), b.size(2));
 }
 
+// What a call writes and what else it reads, by their ranges in memory: tables, lengths and the cache are tensors of their own.
+void separate(const Tensor& written, std::initializer_list<const Tensor*> read) {
+    if (!written.numel()) return;
+    auto bytes = [](const Tensor& t) {
+        int64_t n = 1;
+        for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+        return n * (int64_t)t.element_size();
+    };
+    const char* w = static_cast<const char*>(written.data_ptr());
+    const int64_t size = bytes(written);
+    for (const Tensor* t : read) {
+        if (!t || !t->numel()) continue;
+        const char* r = static_cast<const char*>(t->data_ptr());
+        TORCH_CHECK(w + size <= r || r + bytes(*t) <= w, kOverlap);
+    }
+}
+
 const Tensor* at_or_null(const Maybe& t) { return t ? &*t : nullptr; }
 
 int index(const Tensor& t, int64_t n, const char* name) {
@@ -143,9 +160,11 @@ std::tuple<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& 
         if (k_out) rows(*k_out, "out");
         // an output may be its own input, and shares memory with nothing else that is read or written
         TORCH_CHECK(spread(*q_out) && (same(*q_out, q) || apart(*q_out, q)), kOverlap);
+        separate(*q_out, {&positions, &frequencies});
         if (k) {
             TORCH_CHECK(spread(*k_out) && (same(*k_out, *k) || apart(*k_out, *k)), kOverlap);
             TORCH_CHECK(apart(*q_out, *k) && apart(*k_out, q) && apart(*k_out, *q_out), kOverlap);
+            separate(*k_out, {&positions, &frequencies});
         }
         qo = *q_out;
         ko = k_out;
@@ -168,6 +187,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> plan(const Tensor& le
     const int32_t* add = int32s(fresh, requests, "new_lengths");
     table(block_table, requests);
     TORCH_CHECK(requests <= 1 || block_table.stride(0) >= block_table.size(1), "rows of block_table must not overlap, it is written.");
+    separate(block_table, {&lengths, &fresh, &free_pages, &free_count});
     const int32_t* pages = int32s(free_pages, -1, "free_pages");
     const int32_t* count = int32s(free_count, 1, "free_count");
     TORCH_CHECK(tokens >= 0 && tokens <= kMost, "tokens must be from 0 to 2^31 - 1.");
@@ -193,6 +213,7 @@ void append(const Tensor& cache, const Tensor& k, const Tensor& v, const Tensor&
     const Cache c = cache_of(cache, k.size(2), group_size);
     TORCH_CHECK(k.size(1) == c.kv_heads, "the cache has ", c.kv_heads, " heads, k and v have ", k.size(1), ".");
     const int wide = index(slots, k.size(0), "slots");
+    separate(cache, {&k, &v, &slots});
     c10::cuda::CUDAGuard guard(k.device());
     ok(decdec_kv4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), wide, (uint32_t)k.size(0), c.p, c.pages,
                          c.page_size, c.kv_heads, (uint32_t)k.size(2), (uint32_t)group_size, dt_of(k.scalar_type()), stream_of(k)));
@@ -233,6 +254,7 @@ std::tuple<Tensor, Maybe> attention(const Tensor& q, const Tensor& cache, const 
         TORCH_CHECK(out_given->sizes() == q.sizes() && out_given->scalar_type() == q.scalar_type(), "out must have the shape and type of q.");
         rows(*out_given, "out");
         TORCH_CHECK(spread(*out_given) && apart(*out_given, q), kOverlap);
+        separate(*out_given, {&cache, &block_table, &lengths, &query_starts});
         out = *out_given;
     } else {
         out = empty({tokens, heads, d}, q.scalar_type(), q.device());

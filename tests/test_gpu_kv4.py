@@ -743,6 +743,38 @@ def test_outputs_with_heads_before_tokens(kv4):
         b.run(out=out.flatten()[:448 + 64].as_strided((7, 4, 64), (64, 64, 1)))              # heads that lie over the tokens
 
 
+def test_outputs_over_caches_and_tables_are_refused(kv4):
+    """What a call writes may not lie over the cache, tables, lengths or slots that it reads."""
+    b = Batch(kv4, [40], [4], 4, 2, 64, 64, torch.float16, 16, 674)
+    memory = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    out = memory[:4 * 4 * 64 * 2].view(torch.float16).view(4, 4, 64)
+    over = memory[16:48].view(torch.int32)                             # inside the output's memory
+    lens, table = torch.tensor([40], dtype=torch.int32, device="cuda"), b.table.cuda()
+    q, starts = b.q.cuda(), b.starts.cuda()
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        kv4.attention(q, b.cache, table, lens, starts, 64, out=b.cache.flatten()[:out.numel() * 2].view(torch.float16).view(4, 4, 64))
+    for args in ((over[:table.numel()].view(1, -1), lens, starts), (table, over[:1], starts), (table, lens, over[:2])):
+        with pytest.raises(RuntimeError, match="must not share memory"):
+            kv4.attention(q, b.cache, *args, 64, out=out)
+    frequencies, _ = kv4.rotary_frequencies(64)
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        kv4.rotary(q, None, over[:4], frequencies, out=(out, None))
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        kv4.rotary(q, q[:, :2], torch.zeros(4, dtype=torch.int64, device="cuda"), memory[256:512].view(torch.float64), out=(torch.empty_like(q), out[:, :2]))
+    cache = memory[:16 * R.cell_bytes(64, 64) // 16].view(1, 1, -1)
+    x = memory[64:64 + 128].view(torch.float16).view(1, 1, 64)
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        kv4.append(cache, x, torch.zeros_like(x), torch.zeros(1, dtype=torch.int64, device="cuda"), 64)
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        kv4.append(cache, torch.zeros_like(x), torch.zeros_like(x), over[:1], 64)
+    n = torch.ones(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        kv4.plan(over[1:3], n, over.view(2, 4), n, n[:1], 16, 2)
+    state = torch.zeros(1, 9, dtype=torch.int32, device="cuda")        # a row beside its table is apart from it
+    assert kv4.plan(state[0, :1], n[:1], state[:, 1:], n, n[:1], 16, 1).status.item() == 0
+    assert not memory.any()
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
