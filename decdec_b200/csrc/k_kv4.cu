@@ -328,10 +328,11 @@ template <int D> struct Lanes {
 constexpr uint32_t kRounds = 4;                                     // of a warp at most
 
 // A warp takes a token and `rounds` rounds of its heads, which are coalesced 256-byte reads of keys and values; the group extremes are a
-// few shuffles of (least, -largest) pairs.  Bound by the instructions, 224 for the keys and values of a head of 128: the slot is looked up
-// once for all heads, ties are settled apart.  8191 tokens of 10 heads of 128, written and read back: the slot for every head, divisions and
-// float extremes 84 us, the slot once and packed extremes 51, approximate reciprocals and an exact correction 47; eight elements a lane, and
-// all reads at once, the same.
+// few shuffles of (least, -largest) pairs.  Bound by waiting: two dependent round trips (slot, row), and value codes that lie in pieces of two
+// bytes, four to every 16 bytes and those 64 bytes apart.  Issue slots are 49 % busy (224 instructions for the keys and values of a head of 128),
+// memory 15 %.  8191 tokens of 10 heads of 128, written and read back: the slot for every head, divisions and float extremes 84 us, the slot once
+// and packed extremes 51, approximate reciprocals and an exact correction 47 to 49, steps rounded exactly 50; eight elements a lane, and all reads
+// at once, the same.
 template <int DT, int D, int GS, bool VEC>
 __global__ void __launch_bounds__(256) append_kernel(Rows k, Rows v, const void* slots, int wide, Kv4Cache c, uint32_t tokens, uint32_t chunks, uint32_t rounds,
                                                      unsigned* err) {
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(256) append_kernel(Rows k, Rows v, const void*
 }
 
 // ---- rows out of the cache -----------------------------------------------------------------------------------
-// Bound by memory.  Warps and lanes as in append.
+// Bound by waiting, as append is: issue slots 38 % busy, memory 6 %.  Warps and lanes as in append.
 template <int DT, int D, int GS>
 __global__ void __launch_bounds__(256) gather_kernel(Kv4Cache c, const void* slots, int wide, void* k_out, void* v_out, uint32_t tokens, uint32_t chunks,
                                                      uint32_t rounds, unsigned* err) {

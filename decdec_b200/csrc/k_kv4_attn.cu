@@ -28,7 +28,7 @@ struct Choice {
 // Tiles of 8 rows while a request's rows (queries x heads of a key head) fit one, of 16 up to 64 rows, then of 256; heads of 256 elements
 // have no registers for 16 and no room for 256.  Measured (us; 16 requests of 4096 tokens, 8 key heads of 128) with tiles of 16 / of 256: 32
 // rows 63 / 105, 64 rows 108 / 114, 96 rows 150 / 124; with a step for 32 elements 90 / 108, 160 / 117, 226 / 126; one request of
-// 32768 tokens 39 / 64, 59 / 68, 78 / 73.
+// 32768 tokens 39 / 64, 59 / 68, 78 / 73.  One choice for the batch, by its largest request: the host does not know the others.
 int choose(uint32_t head_dim, uint32_t group, uint32_t ratio, uint32_t max_queries, int dt, Choice* c) {
     const uint64_t rows = (uint64_t)ratio * max_queries;
     c->chunk = head_dim <= 128 && ratio <= (uint32_t)kChunkRows && rows > 64;

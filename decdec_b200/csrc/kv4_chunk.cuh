@@ -4,8 +4,13 @@
 // Per tile and step of 128 tokens, S = Q K^T and O += P V with fp16 operands and fp32 sums in tensor memory.  Keys and values become
 // fp16 numbers on the way (offset + step * code in one rounding, 2^-11, as a gathered cache in 16 bits has; scaled by a power of two per
 // 32 tokens so that both 16-bit types fit), once for the 256 rows of a tile.  Bound by the products and the exponentials: for heads of 128, a step
-// of a tile is 2048 cycles of each; it takes 6100, most of it the chain maximum -> exponentials -> products of a group.  Three requests with
-// chunks of up to 2048 queries at up to 16384 tokens: 1.24 ms, 697 TFLOP/s.
+// of a tile is 2048 cycles of each; it takes 6100, most of it the chain maximum -> exponentials -> products of a group.  17 warps leave a thread 96
+// registers, and every instance spills (152 to 216 bytes of stores).  Three requests with chunks of up to 2048 queries at up to 16384 tokens:
+// 1.24 ms, 697 TFLOP/s.
+//
+// A weight carries the power of two by which its 32 tokens' values are smaller than the largest of the request's steps so far: where that passes 2^14 the
+// fp16 weights are subnormal, and outputs are good to 2^-28 of those largest values a token, whether the row sees them or not.  Sums of
+// weights are fp32 and keep theirs.
 //
 // One block an SM, 17 warps:
 //   warps 0-3, 4-7   rows 0-127 and 128-255 of the tile, a thread a row: queries into shared memory; per step the row's maximum and sum,
@@ -29,7 +34,7 @@ namespace dd {
 
 constexpr int kChunkRows = 256, kChunkStep = 128, kChunkThreads = 17 * 32;
 constexpr float kChunkGrow = 8.0f;
-constexpr int kSegmentSteps = 2;              // what a segment's beginning and end count on the line, in steps (counted as none: 2 % slower)
+constexpr int kSegmentSteps = 2;              // what a segment's beginning and end count on the line, in steps (counted as none: 2 % slower; heads of 128)
 constexpr unsigned kErrWait = 1;
 
 struct ChunkRequest {

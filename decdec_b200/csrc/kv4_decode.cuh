@@ -13,15 +13,17 @@
 //   queries     fp16 after scaling each row to a power of two near 2^9: exact for both 16-bit types (elements below 2^-23 of the row's
 //               largest lose bits)
 //   weights     p_t * step_t in fp16 with the steps scaled by a running power of two per group, so that neither small steps nor
-//               small weights become subnormal before they are 2^-23 of the largest
+//               small weights become subnormal before they are 2^-23 of the largest (the largest step of the cells that the warp has
+//               met, seen by the row or not)
 //   the rest    (scores, running maximum and sum, the middles' part, sums over thread blocks) in fp32
 //
-// Bound by memory and the instructions alike: 390 cycles a cell of 2176 bytes (heads of 128, one group) and scheduler, where the copy rate
-// allows 354.  64 requests of 512 to 16384 tokens, 372 MB: 84 us, 4.4 TB/s.
+// A step of two cells takes a warp 2340 cycles, 390 a cell of 2176 bytes (heads of 128, one group) and scheduler, where the copy rate allows
+// 354; then come the ends of segments.  Neither is full under the profiler: memory 45 %, issue slots 48 %.  64 requests of 512 to 16384 tokens,
+// 372 MB: 84 to 90 us, 4.1 to 4.4 TB/s.
 //
 // The work is a line of cells (16 tokens of one key head), request by request, and every thread block takes an equal part of it
-// (lengths are on the device: each block sums them itself); work that would not fill the device is cut by segments instead.  A warp streams its own cells through shared memory (cp.async, kStages
-// cells ahead) and keeps its own running maximum and sums; the four warps of a block are added where a segment (one request, head and
+// (lengths are on the device: each block sums them itself); work that would not fill the device is cut by segments instead.  A warp streams
+// its own cells through shared memory (cp.async, kStages steps ahead) and keeps its own running maximum and sums; the four warps of a block are added where a segment (one request, head and
 // tile of 8 or 16 query rows) ends.  A segment that blocks share leaves its parts in `part`, and kv4_join adds them.
 #pragma once
 #include "kv4.cuh"
@@ -153,12 +155,13 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4Attn& p, uint32_t b, 
 
 // Pieces of a segment where each has a block to itself: one up to 16 cells (two steps of a warp; a step costs 0.8 us, a join 2), then of 8
 // cells.  One request with 8 key heads, this / blocks of 8 cells cut from the line (us): 16 tokens 6.9 / 31 (one block has all heads), 100 tokens
-// 7.3 / 11.4, 777 tokens 9.7 / 12.5, 3000 tokens 10.3 / 12.9.
+// 7.3 / 11.4, 777 tokens 9.7 / 12.5, 3000 tokens 10.3 / 12.9 (heads of 128).
 __host__ __device__ constexpr int kv4_pieces(int cells) { return cells <= 16 ? 1 : (cells + 7) / 8; }
 
 // What the beginning and the end of a segment (queries, first cells, adding the warps' sums) cost a block, in cells: 5 to 10 thousand cycles
 // at 290 a cell.  Counted as 0 / 16 / 32 / 48 cells: 64 requests of 512 to 16384 tokens 112 / 93 / 84 / 86 us, drafts of 17 requests 104 / 69 / 61
-// / 63: without it the blocks that have the short requests take twice as long as the others.
+// / 63: without it the blocks that have the short requests take twice as long as the others.  Measured with heads of 128; one number for all, though
+// a cell of a head of 64 costs about half as much, one of 256 twice.
 constexpr int kSegmentCells = 32;
 
 // the rows before the first request and behind the last, a row a block at a time

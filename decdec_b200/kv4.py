@@ -9,8 +9,9 @@ A step of a layer, for a batch of requests whose tokens lie one request after an
     kv4.append(cache, k, v, p.slots, group_size)
     y = kv4.attention(q, cache, block_table, p.lengths, p.query_starts, group_size, max_queries=n)
 
-A batch of one with a contiguous cache is a block table that counts up.  Nothing synchronises and every call can be captured in a
-CUDA graph once a call has run eagerly on the device; lengths, tables and slots are read on the device.  Elements are held as
+A batch of one with a contiguous cache is a block table that counts up.  Nothing synchronises but the first append, gather or attention on
+a stream, which allocates its error word; every call can be captured in a CUDA graph once a call has run eagerly on the device; lengths, tables and
+slots are read on the device.  Elements are held as
 offset + step * code with 16 codes and one (step, offset) for `group_size` elements of a head; `include/decdec_b200.h` gives the
 format.  Tensors: fp16 or bf16, [tokens, heads, head_dim], any strides with neighbouring elements in a head.
 """
@@ -128,7 +129,8 @@ def attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, l
     head_dim], which are its last tokens, and lengths[b] tokens in the cache with them.  Query head h reads key head h * kv_heads // heads.
 
     window > 0: each row sees the last `window` tokens up to its own.  A row that sees no token gives zeros.  max_queries: the most rows of a
-    request (default: all rows), which chooses the kernel.  scale: default head_dim ** -0.5.  Rows of no request, before the first or
+    request, which chooses the kernel; the default, all rows, is meant for one request: a decoding batch without it may run on the kernel for
+    prompts, several times slower.  scale: default head_dim ** -0.5.  Rows of no request, before the first or
     behind the last, are left as they are in `out`, zeros where `out` is not given.  return_lse: also the fp32 logarithms [tokens, heads] of the sums of exp(scale q k^T)."""
     out, lse = _kv4.attention(q, cache, block_table, lengths, query_starts, group_size, max_queries, scale, window, out, return_lse)
     return (out, lse) if return_lse else out

@@ -316,7 +316,8 @@ __all__ = [
 
 def stream_status() -> int:
     """Error word of the current stream's workspace (0 = fine; 1 = a bounded wait inside a kernel ran out,
-    2 = a launch did not get the shared-memory layout it was sized for).  Does not synchronise."""
+    2 = a launch did not get the shared-memory layout it was sized for, 3 = a page, a slot or a length outside the 4-bit cache).  Does not
+    synchronise."""
     err = C.c_uint32(0)
     _call("decdec_stream_status", _stream(), C.byref(err))
     return int(err.value)
