@@ -36,6 +36,7 @@ constexpr int kChunkRows = 256, kChunkStep = 128, kChunkThreads = 17 * 32;
 constexpr float kChunkGrow = 8.0f;
 constexpr int kSegmentSteps = 2;              // what a segment's beginning and end count on the line, in steps (counted as none: 2 % slower; heads of 128)
 constexpr unsigned kErrWait = 1;
+constexpr long long kWaitClocks = 1000000000;    // about half a second
 
 struct ChunkRequest {
     int start, queries, length, tiles, per_tile;         // per_tile: queries of a tile
@@ -130,13 +131,13 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded: after about half a second the block gives up, here and in every later wait.
+// Bounded: then the block gives up, here and in every later wait.
 __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, unsigned* err) {
     if (bar_try(bar, parity)) return;
     const long long t0 = clock64();
     while (!bar_try(bar, parity)) {
         if (*gave_up) return;
-        if (clock64() - t0 > 1000000000ll) {
+        if (clock64() - t0 > kWaitClocks) {
             *gave_up = 1u;
             raise_error(err, kErrWait);
             return;
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
     constexpr uint32_t CELL = kv4_cell_bytes(D, GS);
     constexpr int LW = D / 32;                                                   // 16-byte loads of a lane's keys (and values) in a step
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[14];
+    __shared__ uint64_t bars[15];
     __shared__ uint32_t s_tmem, s_gave_up;
     __shared__ ChunkMeta s_meta[4];
     __shared__ long long s_sum[17];
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t bar0 = smem_at(bars);
     const uint32_t bar_k = bar0, bar_kfree = bar0 + 16, bar_v = bar0 + 32, bar_vfree = bar0 + 48, bar_s = bar0 + 64, bar_p = bar0 + 80, bar_o = bar0 + 96;
-    const uint32_t bar_q = bar0 + 104;                                           // one for the outputs of both groups, one for the queries
+    const uint32_t bar_q = bar0 + 104, bar_end = bar0 + 112;                     // one for the outputs of both groups, the queries, the end
     volatile uint32_t* gave_up = &s_gave_up;
 
     if (warp == 16) {
@@ -194,6 +195,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
         }
         bar_init(bar_o, 1);                                                      // both groups' outputs end together
         bar_init(bar_q, 8);
+        bar_init(bar_end, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_trigger();
@@ -343,6 +345,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(Kv4Attn p) 
                 products_done(bar_o);
                 ++seg;
             }
+            // A block that gave up issued products that nobody waits for: they end before the tensor memory is freed and the block leaves.
+            products_done(bar_end);
+            const long long t0 = clock64();
+            while (!bar_try(bar_end, 0u) && clock64() - t0 < kWaitClocks) {}
         }
         __syncwarp();
     } else if (warp >= 8) {
