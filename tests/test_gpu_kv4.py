@@ -775,6 +775,25 @@ def test_outputs_over_caches_and_tables_are_refused(kv4):
     assert not memory.any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window", [0, 700])
+def test_many_queries_of_wide_heads_at_length(kv4, dtype, window):
+    b = Batch(kv4, [1500, 900], [90, 33], 8, 1, 256, 128, dtype, 48, 2200)
+    out, lse = b.run(window=window, return_lse=True)
+    assert not b.dense
+    b.check(out, lse, window=window)
+    assert torch.equal(out, b.run(window=window))
+
+
+@pytest.mark.parametrize("most,dense", [(None, True), (260, True), (1, False)])
+def test_long_decoding_requests_beside_a_prompt(kv4, most, dense):
+    lengths, queries = [4000, 2777, 3100, 5000], [1, 260, 1, 5]
+    b = Batch(kv4, lengths, queries, 8, 2, 64, 64, torch.float16, 32, 2300)
+    out, lse = b.run(return_lse=True, **({} if most is None else {"max_queries": most}))
+    assert b.dense == dense
+    b.check(out, lse)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,d,group,interleaved", [(torch.bfloat16, 128, 128, False), (torch.float16, 64, 32, True)])
